@@ -58,7 +58,7 @@ def stale(out: Path, deps: list[Path]) -> bool:
 
 def main() -> None:
     force = "--force" in sys.argv
-    if not REF.exists():
+    if not (REF / "sched" / "src").is_dir():
         print(f"reference tree {REF} not present; keeping prebuilt oracle/_ref as is")
         return
     OBJ.mkdir(parents=True, exist_ok=True)

@@ -282,7 +282,7 @@ def build_oracle_ref(force: bool = False, verbose: bool = False) -> Path | None:
     if not script.exists():
         return None
     ref = Path(os.environ.get("XSCHED_REFERENCE_DIR", "/root/reference"))
-    if not ref.exists():
+    if not (ref / "sched" / "src").is_dir():          # no tree, or an empty mount point
         return None
     cmd = [sys.executable, str(script)] + (["--force"] if force else [])
     _run(cmd, verbose)
