@@ -53,6 +53,8 @@ typedef enum {
     XPK_KIND_VECADD = 2,  /* c[i] = a[i] + b[i], fp32                              */
     XPK_KIND_SORT   = 3,  /* int32 ascending LSD radix sort, 8-bit digits          */
     XPK_KIND_GEMM   = 4,  /* bf16 C[M,N] = A[M,K] * B[N,K]^T, fp32 accumulate      */
+    XPK_KIND_ATTENTION = 5, /* attention over a paged key/value cache              */
+    XPK_KIND_KV_COPY = 6, /* copies of pages of a key/value cache                  */
 } xpkKind;
 
 /* Launch-time flags for xpkTaskCreate*. */
@@ -202,8 +204,138 @@ xpkResult xpkTaskDestroy(xpkTask_t task);
 #define XPK_SORT_NOALLOC_MAX_KEYS (4ull << 20)
 xpkResult xpkSortNoAlloc(int32_t *keys, int32_t *tmp, uint64_t n, void *stream);
 
-/* Kernels launched by this library in this process since load (all tasks, and the sort kernels
- * of xpkSortNoAlloc). */
+/* ---- paged key/value cache -------------------------------------------------------------
+ * (No counterpart in the reference, which has no model kernels.)
+ *
+ * The operators of a decode loop around one cache: room for new tokens, forks that share pages, copies, compaction;
+ * the norms, rotation and write of new queries, keys and values; the attention that reads them, with a prefix that a
+ * batch shares read once for all.  The arrays belong to the caller and stay where they are for the cache's life:
+ *
+ *   k, v        [layers][pages][kv_heads][page_size][head_dim], bf16 or fp16, 16-byte aligned
+ *   page_table  [seqs][table_width] page ids, position p of a sequence lies on entry p / page_size
+ *   lens        [seqs] positions that a sequence holds (0 = the slot is free)
+ *   refs        [pages] how many table entries name a page (0 = the page is free)
+ *
+ * page_size is 16, 32, 64 or 128, head_dim 64 or 128.  The three integer arrays live on the device, and every call
+ * reads what they hold when its kernels run, so a loop can be captured once and replayed while lengths grow.  Page ids
+ * and sequence ids are checked by the kernels: a sequence outside [0, seqs) is padding and is passed over, a page
+ * outside [0, pages) is treated as not there (never read, never written).
+ *
+ * Calls are asynchronous on `stream`, a stream of the cache's device (the device current at creation), which is made
+ * current for the call.  Calls on one cache share the handle's workspace (fork, extend, compact) and the arrays above:
+ * those that change them are ordered by the caller, on one stream or by events.                                    */
+typedef enum {
+    XPK_DTYPE_BF16 = 1,
+    XPK_DTYPE_F16  = 2,
+} xpkDtype;
+
+typedef struct xpkKvCache_st *xpkKvCache_t;
+
+typedef struct {
+    void *k, *v;
+    int32_t *page_table, *lens, *refs;
+    uint32_t dtype;                                   /* xpkDtype */
+    uint32_t layers, pages, kv_heads, page_size, head_dim, seqs, table_width;
+} xpkKvCacheDesc;
+
+/* Checks the description and allocates the handle's workspace (12 bytes per page and 8 KB on the device). */
+xpkResult xpkKvCacheCreate(xpkKvCache_t *cache, const xpkKvCacheDesc *desc);
+xpkResult xpkKvCacheDestroy(xpkKvCache_t cache);
+
+/* At most this many entries in the lists of fork and extend. */
+#define XPK_KV_MAX_LIST 2048
+
+/* The listed sequences give their pages back and are empty afterwards (lens 0, their table entries -1).  A sequence
+ * listed twice, and one that is empty, is passed over. */
+xpkResult xpkKvFree(xpkKvCache_t cache, const int32_t *seqs, uint32_t n, void *stream);
+
+/* children[i] becomes a copy of parents[i] that shares its pages (no page is copied here; extend copies the last one
+ * when one of its holders grows).  A child has to be empty before the call: entries with a child that is not, with an
+ * empty parent, or with a child that an earlier entry has taken are passed over. */
+xpkResult xpkKvFork(xpkKvCache_t cache, const int32_t *parents, const int32_t *children, uint32_t n, void *stream);
+
+/* Makes room for tokens[i] more positions of seqs[i] and adds them to lens.  New pages are the free ones of lowest
+ * index, in the order of the list; a last page that is partly filled and that others hold too is copied (all layers)
+ * to a new page first, except by the list's last holder once nobody else is left.  A sequence counts once, at its first
+ * place in the list.  All or nothing: if pages are missing, or a sequence would pass the table's width, nothing changes;
+ * xpkKvResult tells. */
+xpkResult xpkKvExtend(xpkKvCache_t cache, const int32_t *seqs, const int32_t *tokens, uint32_t n, void *stream);
+
+/* Moves the live pages of highest index into the holes below them until the pages in use are [0, live), ascending to
+ * ascending, and rewrites table and refs.  Only the first ceil(lens / page_size) entries of a table row are looked at. */
+xpkResult xpkKvCompact(xpkKvCache_t cache, void *stream);
+
+/* Copies page src[i] to page dst[i] in all layers.  No page may be in both lists, or twice in dst. */
+xpkResult xpkKvCopy(xpkKvCache_t cache, const int32_t *src, const int32_t *dst, uint32_t n, void *stream);
+/* The same as a preemptible task; a tile is 64 KB. */
+xpkResult xpkTaskCreateKvCopy(xpkTask_t *task, xpkKvCache_t cache, const int32_t *src, const int32_t *dst, uint32_t n,
+                              uint32_t flags, uint32_t *flag_dev);
+
+/* What the last extend or compact found, read back on `stream` (which it waits for). */
+typedef struct {
+    int32_t copied;    /* pages copied (extend) or moved (compact)                          */
+    int32_t missing;   /* extend: pages short; nothing was changed when not 0              */
+    int32_t refused;   /* extend: sequences that would pass the table's width (as above)   */
+    int32_t live;      /* compact: pages in use                                             */
+} xpkKvReport;
+xpkResult xpkKvResult(xpkKvCache_t cache, xpkKvReport *report, void *stream);
+
+/* Norms, rotation and write of new tokens, one pass over the rows of a projection.
+ *
+ * Row r of `qkv` holds q_heads queries, kv_heads keys and kv_heads values of head_dim elements each.  The rows
+ * starts[i] .. starts[i+1] are the last ones of sequence seqs[i] (after extend): row j of t has position
+ * lens - t + j.  Queries and keys are divided by their root mean square over the head (eps added to the mean) and
+ * multiplied by q_weight / k_weight [head_dim], in fp32 (NULL: no norm); then the first `rotary` elements are turned by
+ * position * inv_freq[j] (angles in fp64): the pairs are (j, j + rotary / 2), or (2j, 2j + 1) with `interleaved`; one
+ * rounding at the end.  Queries go to `q` [rows][q_heads][head_dim], keys and values to the cache's `layer`.
+ * Rows of padded sequences, rows before position 0 and rows behind starts[n] stay as they are.  A key whose page is
+ * missing is not written. */
+typedef struct {
+    void *q;
+    const void *qkv;
+    uint64_t q_stride, qkv_stride;      /* elements between rows; 0 = dense, else a multiple of 8                  */
+    const int32_t *seqs;                /* [n]; NULL: sequence i                                                  */
+    const int32_t *starts;              /* [n + 1] ascending; NULL: one row per sequence                          */
+    const void *q_weight, *k_weight;
+    const double *inv_freq;             /* [rotary / 2] on the device                                             */
+    float eps;
+    uint32_t n, rows, q_heads, layer, rotary, interleaved;   /* rotary: a multiple of 16 up to head_dim, 0 = none */
+} xpkKvAppendArgs;
+xpkResult xpkKvAppend(xpkKvCache_t cache, const xpkKvAppendArgs *args, void *stream);
+
+/* Attention of the rows of `q` (laid out and assigned to sequences as above) to the positions of their own sequences
+ * up to and with their own: out = softmax(scale * q k^T) v, fp32 accumulation and softmax.  Query heads
+ * h * q_heads / kv_heads ... read key head h.
+ *
+ * `shared_len` (one word on the device, or NULL) promises that the first so many positions lie on the same pages in
+ * all sequences of the call that are longer than that; those pages are then read once for all instead of once per
+ * sequence.  The result is the one without it up to rounding.  A row that sees nothing is written as zeros; rows of
+ * padded sequences and behind starts[n] stay as they are.
+ *
+ * `scratch`: xpkAttentionScratchBytes bytes, 256-byte aligned, zeroed once before its first use; a call leaves it ready
+ * for the next.  Calls that may overlap on the GPU (other streams, other captured graphs) need scratch of their own.
+ * A call that was refused wrote nothing.  n <= XPK_ATTENTION_MAX_SEQS. */
+#define XPK_ATTENTION_MAX_SEQS 1024
+typedef struct {
+    void *out;
+    const void *q;
+    uint64_t out_stride, q_stride;      /* elements between rows; 0 = dense, else a multiple of 8                  */
+    const int32_t *seqs, *starts;
+    const int32_t *shared_len;
+    void *scratch;
+    uint64_t scratch_bytes;
+    float scale;
+    uint32_t n, rows, q_heads, layer;
+} xpkAttentionArgs;
+size_t    xpkAttentionScratchBytes(xpkKvCache_t cache, uint32_t rows, uint32_t n, uint32_t q_heads);
+xpkResult xpkAttention(xpkKvCache_t cache, const xpkAttentionArgs *args, void *stream);
+/* The same as a preemptible task.  Its scratch is its own, and is cleared here.  Lengths and tables are not to change between a
+ * launch that was preempted and the one that finishes it. */
+xpkResult xpkTaskCreateAttention(xpkTask_t *task, xpkKvCache_t cache, const xpkAttentionArgs *args, uint32_t flags,
+                                 uint32_t *flag_dev);
+
+/* Kernels launched by this library in this process since load (all tasks, the sort kernels of xpkSortNoAlloc, and
+ * the cache's calls). */
 uint64_t xpkLaunchCount(void);
 
 #ifdef __cplusplus

@@ -355,6 +355,8 @@ static EncodeTiledFn get_encode_fn() {
     return fn;
 }
 
+void *tensor_map_encoder() { return (void *)get_encode_fn(); }
+
 // rows x cols bf16, row-major (cols contiguous); box = box_rows x 64 columns, 128-byte swizzle.
 int gemm_make_map(void *map_out, const void *base, uint64_t rows, uint64_t cols, uint32_t box_rows) {
     EncodeTiledFn fn = get_encode_fn();

@@ -1,7 +1,6 @@
 // C ABI of the preemptible-kernel library (declared in include/xsched_b200/pk.h).
 // Host-side bookkeeping only: control-block allocation, launch geometry, mailbox reads.
-#include "xsched_b200/pk.h"
-#include "pk_common.cuh"
+#include "kv_cache.cuh"
 
 #include <cuda.h>
 #include <algorithm>
@@ -37,38 +36,15 @@ cudaError_t gemm_pair_prepare();
 unsigned long long gemm_pair_tiles(uint32_t M, uint32_t N);
 cudaError_t launch_gemm_pair(bool preemptible, bool abort_inflight, Ctl *ctl, const void *map_a, const void *map_b, void *C,
                              uint32_t M, uint32_t N, uint32_t K, unsigned long long launch_no, int grid, cudaStream_t stream);
+// attention.cu, kv_pages.cu
+cudaError_t launch_attention(bool preemptible, Ctl *ctl, const xpkKvCache_st *cache, const xpkAttentionArgs &x, unsigned long long launch_no,
+                             int grid, cudaStream_t st);
+cudaError_t launch_kv_copy_task(bool preemptible, Ctl *ctl, const CacheView &c, const int32_t *src, const int32_t *dst, uint32_t n,
+                                unsigned long long launch_no, int sms, cudaStream_t st);
 } // namespace xpk
 
 using xpk::Ctl;
 using xpk::Mailbox;
-
-struct xpkTask_st {
-    uint32_t kind = 0;
-    uint32_t flags = 0;
-    int device = 0;
-    int sm_count = 0;
-    Ctl *ctl = nullptr;               // device
-    Mailbox *mb_host = nullptr;       // mapped pinned host memory
-    Mailbox *mb_dev = nullptr;        // device alias
-    uint32_t *flag = nullptr;         // flag the kernels poll
-    unsigned long long total = 0;
-    // Written by whichever thread launches or resets the task (an XQueue worker, the scheduler's thread on a
-    // relaunch), read by application threads in xpkTaskQuery / xpkTaskWait.
-    std::atomic<unsigned long long> launches{0};        // launch counter echoed by the mailbox
-    std::atomic<unsigned long long> reset_at{0};        // value of `launches` at the last reset
-    std::atomic<cudaStream_t> last_stream{nullptr};     // stream of the most recent launch
-    // operands
-    void *p0 = nullptr; const void *p1 = nullptr; const void *p2 = nullptr;
-    float s = 0.f;
-    unsigned long long n = 0;
-    unsigned long long tile_elems = 0;
-    uint32_t *sort_hist = nullptr, *sort_state = nullptr;
-    size_t sort_scratch_bytes = 0;
-    uint32_t M = 0, N = 0, K = 0;
-    bool gemm_pair = false;           // the two-CTA form (tensor maps with 128-row boxes)
-    alignas(64) unsigned char map_a[128];
-    alignas(64) unsigned char map_b[128];
-};
 
 namespace {
 
@@ -120,25 +96,14 @@ DeviceState *device_state(int *dev_out) {
     return &d;
 }
 
-// Makes the task's device current for the duration of a call and puts the caller's device back.  The
-// entry points that take a task may be called from any thread (a worker thread that never called
-// cudaSetDevice is on device 0), while the task's memory and streams belong to the device it was
-// created on.
-class DeviceGuard {
-public:
-    explicit DeviceGuard(int device) {
-        if (cudaGetDevice(&prev_) != cudaSuccess) { prev_ = -1; return; }
-        if (prev_ != device) { if (cudaSetDevice(device) == cudaSuccess) switched_ = true; }
-    }
-    ~DeviceGuard() { if (switched_) cudaSetDevice(prev_); }
-    DeviceGuard(const DeviceGuard &) = delete;
-    DeviceGuard &operator=(const DeviceGuard &) = delete;
-private:
-    int prev_ = -1;
-    bool switched_ = false;
-};
+} // namespace
 
-bool aligned16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
+namespace xpk {
+
+int device_sms() {
+    DeviceState *d = device_state(nullptr);
+    return d ? d->sm_count : 0;
+}
 
 xpkResult task_common(xpkTask_st *t, uint32_t kind, uint32_t flags, unsigned long long total, uint32_t *flag_dev) {
     DeviceState *d = device_state(&t->device);
@@ -166,7 +131,13 @@ void task_free(xpkTask_st *t) {
     delete t;
 }
 
-} // namespace
+} // namespace xpk
+
+using xpk::DeviceGuard;
+using xpk::aligned16;
+using xpk::view_of;
+using xpk::task_common;
+using xpk::task_free;
 
 extern "C" {
 
@@ -395,6 +366,13 @@ xpkResult xpkTaskLaunch(xpkTask_t t, void *stream, int sm_limit) {
         e = xpk::launch_gemm(preemptible, (t->flags & XPK_FLAG_ABORT_INFLIGHT) != 0, t->ctl, t->map_a, t->map_b, t->p0,
                              t->M, t->N, t->K, launch_no, (int)grid, s);
         break;
+    case XPK_KIND_ATTENTION:
+        e = xpk::launch_attention(preemptible, t->ctl, t->cache, t->attention, launch_no, sms, s);
+        break;
+    case XPK_KIND_KV_COPY:
+        e = xpk::launch_kv_copy_task(preemptible, t->ctl, view_of(t->cache), (const int32_t *)t->p1, (const int32_t *)t->p2, (uint32_t)t->n,
+                                     launch_no, sms, s);
+        break;
     default:
         return XPK_ERR_INVALID_VALUE;
     }
@@ -411,7 +389,7 @@ xpkResult xpkTaskQuery(xpkTask_t t, xpkTaskInfo *info) {
     const unsigned long long launches = t->launches.load(), reset_at = t->reset_at.load();
     const unsigned long long seq = m->seq;
     std::atomic_thread_fence(std::memory_order_acquire);
-    info->tiles_total = t->total;
+    info->tiles_total = t->kind == XPK_KIND_ATTENTION && seq > 0 ? m->tiles_total : t->total;   // attention: counted by the kernel
     info->launches = launches;
     if (launches == reset_at) {                  // nothing launched since creation / reset
         info->status = XPK_STATUS_IDLE;
@@ -476,6 +454,7 @@ xpkResult xpkTaskReset(xpkTask_t t, void *stream) {
     const unsigned long long launches = t->launches.load();
     const bool at_start = launches == t->reset_at.load() || (m->seq == launches && m->status == XPK_STATUS_COMPLETED);
     if (!at_start && cudaMemsetAsync(t->ctl, 0, xpk::kCtlResetBytes, s) != cudaSuccess) return XPK_ERR_CUDA;
+    if (t->clear_bytes && !at_start && cudaMemsetAsync(t->clear_at, 0, t->clear_bytes, s) != cudaSuccess) return XPK_ERR_CUDA;
     if (t->kind == XPK_KIND_SORT) {
         if (cudaMemsetAsync(t->sort_hist, 0, t->sort_scratch_bytes, s) != cudaSuccess) return XPK_ERR_CUDA;
     }

@@ -154,16 +154,19 @@ __device__ __forceinline__ void raise_error(Ctl *ctl, uint32_t code) {
 
 // Called by one thread per CTA after all of the CTA's global writes are ordered before it
 // (the caller does __syncthreads(); this function fences).  `done_by_cta` = tiles this CTA
-// finished in this launch; `launch_no` = the host's launch counter for this task, echoed
-// into the mailbox so the host can tell this launch's result from the previous one's.  The last CTA to arrive folds the launch into the cursor.
-__device__ __forceinline__ void cta_exit(Ctl *ctl, unsigned long long done_by_cta,
-                                         unsigned long long launch_no) {
+// finished in this launch.  True for the last CTA to arrive, which then calls cta_fold.
+__device__ __forceinline__ bool cta_leave(Ctl *ctl, unsigned long long done_by_cta) {
     if (done_by_cta) atomicAdd(&ctl->tiles_done, done_by_cta);
     __threadfence();
     const uint32_t prev = atomicAdd(&ctl->ctas_exited, 1u);
-    if (prev + 1u != gridDim.x) return;
+    if (prev + 1u != gridDim.x) return false;
     __threadfence();
+    return true;
+}
 
+// Folds the launch into the cursor and publishes its outcome.  `launch_no` = the host's launch counter for
+// this task, echoed into the mailbox so the host can tell this launch's result from the previous one's.
+__device__ __forceinline__ void cta_fold(Ctl *ctl, unsigned long long launch_no) {
     volatile Ctl *v = ctl;
     const unsigned long long nret   = v->n_returned;
     const unsigned long long fresh  = v->total - v->base;
@@ -215,6 +218,11 @@ __device__ __forceinline__ void cta_exit(Ctl *ctl, unsigned long long done_by_ct
         m->seq = launch_no;
         __threadfence_system();
     }
+}
+
+// The usual end of a kernel: leave, and fold if this was the last CTA.
+__device__ __forceinline__ void cta_exit(Ctl *ctl, unsigned long long done_by_cta, unsigned long long launch_no) {
+    if (cta_leave(ctl, done_by_cta)) cta_fold(ctl, launch_no);
 }
 
 } // namespace xpk

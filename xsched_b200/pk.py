@@ -18,7 +18,9 @@ lib = C.CDLL(str(_LIB_PATH))
 
 SUCCESS = 0
 STATUS_IDLE, STATUS_RUNNING, STATUS_COMPLETED, STATUS_PREEMPTED, STATUS_ERROR = range(5)
-KIND_TRIAD, KIND_VECADD, KIND_SORT, KIND_GEMM = 1, 2, 3, 4
+KIND_TRIAD, KIND_VECADD, KIND_SORT, KIND_GEMM, KIND_ATTENTION, KIND_KV_COPY = 1, 2, 3, 4, 5, 6
+DTYPE_BF16, DTYPE_F16 = 1, 2
+KV_MAX_LIST, ATTENTION_MAX_SEQS = 2048, 1024
 FLAG_NONE, FLAG_NON_PREEMPTIBLE, FLAG_ABORT_INFLIGHT, FLAG_GEMM_ONE_CTA, FLAG_GEMM_CTA_PAIR = 0, 1, 2, 4, 8
 
 #: every symbol include/xsched_b200/pk.h declares
@@ -28,6 +30,8 @@ EXPORTS = [
     "xpkTaskCreateGemm", "xpkTaskLaunch", "xpkTaskQuery", "xpkTaskWait", "xpkTaskReset",
     "xpkTaskFlag", "xpkTaskKind", "xpkTaskDestroy", "xpkLaunchCount", "xpkSortNoAlloc", "xpkTaskTimes",
     "xpkFlagAttachRelay", "xpkFlagDetachRelay",
+    "xpkKvCacheCreate", "xpkKvCacheDestroy", "xpkKvFree", "xpkKvFork", "xpkKvExtend", "xpkKvCompact", "xpkKvCopy",
+    "xpkTaskCreateKvCopy", "xpkKvResult", "xpkKvAppend", "xpkAttentionScratchBytes", "xpkAttention", "xpkTaskCreateAttention",
 ]
 
 
@@ -37,6 +41,28 @@ class TaskInfo(C.Structure):
 
 
 _vp, _u32, _u64 = C.c_void_p, C.c_uint32, C.c_uint64
+
+
+class KvCacheDesc(C.Structure):
+    _fields_ = [("k", _vp), ("v", _vp), ("page_table", _vp), ("lens", _vp), ("refs", _vp), ("dtype", _u32), ("layers", _u32), ("pages", _u32),
+                ("kv_heads", _u32), ("page_size", _u32), ("head_dim", _u32), ("seqs", _u32), ("table_width", _u32)]
+
+
+class KvReport(C.Structure):
+    _fields_ = [("copied", C.c_int32), ("missing", C.c_int32), ("refused", C.c_int32), ("live", C.c_int32)]
+
+
+class KvAppendArgs(C.Structure):
+    _fields_ = [("q", _vp), ("qkv", _vp), ("q_stride", _u64), ("qkv_stride", _u64), ("seqs", _vp), ("starts", _vp), ("q_weight", _vp), ("k_weight", _vp),
+                ("inv_freq", _vp), ("eps", C.c_float), ("n", _u32), ("rows", _u32), ("q_heads", _u32), ("layer", _u32), ("rotary", _u32),
+                ("interleaved", _u32)]
+
+
+class AttentionArgs(C.Structure):
+    _fields_ = [("out", _vp), ("q", _vp), ("out_stride", _u64), ("q_stride", _u64), ("seqs", _vp), ("starts", _vp), ("shared_len", _vp), ("scratch", _vp),
+                ("scratch_bytes", _u64), ("scale", C.c_float), ("n", _u32), ("rows", _u32), ("q_heads", _u32), ("layer", _u32)]
+
+
 lib.xpkResultString.restype = C.c_char_p
 lib.xpkResultString.argtypes = [C.c_int]
 lib.xpkDeviceSmCount.argtypes = [C.POINTER(C.c_int)]
@@ -62,6 +88,20 @@ lib.xpkTaskDestroy.argtypes = [_vp]
 lib.xpkLaunchCount.restype = _u64
 lib.xpkSortNoAlloc.argtypes = [_vp, _vp, _u64, _vp]
 SORT_NOALLOC_MAX_KEYS = 4 << 20
+lib.xpkKvCacheCreate.argtypes = [C.POINTER(_vp), C.POINTER(KvCacheDesc)]
+lib.xpkKvCacheDestroy.argtypes = [_vp]
+lib.xpkKvFree.argtypes = [_vp, _vp, _u32, _vp]
+lib.xpkKvFork.argtypes = [_vp, _vp, _vp, _u32, _vp]
+lib.xpkKvExtend.argtypes = [_vp, _vp, _vp, _u32, _vp]
+lib.xpkKvCompact.argtypes = [_vp, _vp]
+lib.xpkKvCopy.argtypes = [_vp, _vp, _vp, _u32, _vp]
+lib.xpkTaskCreateKvCopy.argtypes = [C.POINTER(_vp), _vp, _vp, _vp, _u32, _u32, _vp]
+lib.xpkKvResult.argtypes = [_vp, C.POINTER(KvReport), _vp]
+lib.xpkKvAppend.argtypes = [_vp, C.POINTER(KvAppendArgs), _vp]
+lib.xpkAttentionScratchBytes.restype = C.c_size_t
+lib.xpkAttentionScratchBytes.argtypes = [_vp, _u32, _u32, _u32]
+lib.xpkAttention.argtypes = [_vp, C.POINTER(AttentionArgs), _vp]
+lib.xpkTaskCreateAttention.argtypes = [C.POINTER(_vp), _vp, C.POINTER(AttentionArgs), _u32, _vp]
 
 
 class XpkError(RuntimeError):
@@ -173,6 +213,24 @@ class Task:
                                      flag.ptr if flag else None), "xpkTaskCreateGemm")
         return Task(h.value, (a, b, c, flag))
 
+    @staticmethod
+    def attention(cache: "KvCache", out, q, seqs, *, scratch, starts=None, shared_len=None, layer: int = 0, scale: float | None = None,
+                  flags: int = 0, flag: Flag | None = None) -> "Task":
+        """KvCache.attention as a task; `scratch` is the task's own.  Its tiles are counted when a launch has read the lengths."""
+        a = cache._attention_args(out, q, seqs, starts, shared_len, scratch, layer, scale)
+        h = _vp()
+        _check(lib.xpkTaskCreateAttention(C.byref(h), cache.handle, C.byref(a), flags, flag.ptr if flag else None), "xpkTaskCreateAttention")
+        return Task(h.value, (cache, out, q, seqs, starts, shared_len, scratch, flag))
+
+    @staticmethod
+    def kv_copy(cache: "KvCache", src, dst, flags: int = 0, flag: Flag | None = None) -> "Task":
+        """KvCache.copy as a task."""
+        n = cache._list("kv_copy", src, dst)
+        h = _vp()
+        _check(lib.xpkTaskCreateKvCopy(C.byref(h), cache.handle, src.data_ptr(), dst.data_ptr(), n, flags, flag.ptr if flag else None),
+               "xpkTaskCreateKvCopy")
+        return Task(h.value, (cache, src, dst, flag))
+
     # -- control ------------------------------------------------------------------------
     def launch(self, stream: int, sm_limit: int = 0) -> None:
         _check(lib.xpkTaskLaunch(self.handle, stream, sm_limit), "xpkTaskLaunch")
@@ -203,3 +261,153 @@ class Task:
             lib.xpkTaskDestroy(self.handle)
             self.handle = None
             self._keep = ()
+
+
+def _rows(what: str, x, width: int):
+    """(rows, elements between rows) of a tensor whose trailing dimensions, `width` elements in all, are dense."""
+    rows = x.shape[0]
+    if x.numel() != rows * width:
+        raise ValueError(f"{what}: {tuple(x.shape)} is not [rows] of {width} elements")
+    if x.is_contiguous():
+        return rows, 0
+    inner = 1
+    for size, stride in zip(reversed(x.shape[1:]), reversed(x.stride()[1:])):
+        if size != 1 and stride != inner:
+            raise ValueError(f"{what}: a row's elements lie apart (strides {x.stride()})")
+        inner *= size
+    return rows, x.stride(0) if rows > 1 else 0
+
+
+class KvCache:
+    """A paged key/value cache and the operators of a decode loop around it (see pk.h for what each does exactly).
+
+    k, v [layers, pages, kv_heads, page_size, head_dim] (bf16 or fp16), page_table [seqs, width], lens [seqs] and refs [pages]
+    (int32) are the caller's tensors on one device and stay where they are.  Calls take the stream they run on; lists and
+    lengths are read on the device when the kernels run.  destroy() gives the handle back."""
+
+    def __init__(self, k, v, page_table, lens, refs):
+        dtype = {"torch.bfloat16": DTYPE_BF16, "torch.float16": DTYPE_F16}.get(str(k.dtype))
+        if dtype is None or k.dtype != v.dtype:
+            raise ValueError(f"k and v are both bfloat16 or both float16, got {k.dtype} and {v.dtype}")
+        if k.dim() != 5 or k.shape != v.shape:
+            raise ValueError(f"k and v are [layers, pages, kv_heads, page_size, head_dim] alike, got {tuple(k.shape)} and {tuple(v.shape)}")
+        layers, pages, heads, page, dim = k.shape
+        if page_table.dim() != 2 or lens.shape != page_table.shape[:1] or refs.shape != (pages,):
+            raise ValueError("page_table is [seqs, width], lens [seqs], refs [pages]")
+        for name, x in (("page_table", page_table), ("lens", lens), ("refs", refs)):
+            if str(x.dtype) != "torch.int32":
+                raise ValueError(f"{name} is int32, got {x.dtype}")
+        for name, x in (("k", k), ("v", v), ("page_table", page_table), ("lens", lens), ("refs", refs)):
+            if not x.is_contiguous() or x.device != k.device or not x.is_cuda:
+                raise ValueError(f"{name} is contiguous and on the same CUDA device as k")
+        self.k, self.v, self.page_table, self.lens, self.refs = k, v, page_table, lens, refs
+        self.device, self.dtype, self.heads, self.dim = k.device, k.dtype, heads, dim
+        self.handle = None
+        d = KvCacheDesc(k.data_ptr(), v.data_ptr(), page_table.data_ptr(), lens.data_ptr(), refs.data_ptr(), dtype, layers, pages, heads, page, dim,
+                        page_table.shape[0], page_table.shape[1])
+        h = _vp()
+        import torch
+        with torch.cuda.device(k.device):                     # the handle belongs to the device that is current here
+            _check(lib.xpkKvCacheCreate(C.byref(h), C.byref(d)), "xpkKvCacheCreate")
+        self.handle = h.value
+
+    def destroy(self) -> None:
+        if self.handle:
+            lib.xpkKvCacheDestroy(self.handle)
+            self.handle = None
+
+    # -- checks -------------------------------------------------------------------------
+    def _ints(self, what: str, x):
+        if x is None:
+            return None
+        if str(x.dtype) != "torch.int32" or not x.is_contiguous() or x.device != self.device:
+            raise ValueError(f"{what} is a contiguous int32 tensor on {self.device}")
+        return x.data_ptr()
+
+    def _list(self, what: str, a, b) -> int:
+        if self._ints(what, a) is None or self._ints(what, b) is None or a.numel() != b.numel():
+            raise ValueError(f"{what}: two int32 lists of the same length")
+        return a.numel()
+
+    def _data(self, what: str, x):
+        if x is None:
+            return None
+        if x.dtype != self.dtype or x.device != self.device:
+            raise ValueError(f"{what} is {self.dtype} on {self.device}, got {x.dtype} on {x.device}")
+        return x.data_ptr()
+
+    def _entries(self, seqs, starts, rows: int) -> int:
+        n = seqs.numel() if seqs is not None else starts.numel() - 1 if starts is not None else rows
+        if starts is not None and starts.numel() != n + 1:
+            raise ValueError(f"starts has {starts.numel()} entries for {n} sequences: one more is wanted")
+        if starts is None and n != rows:
+            raise ValueError(f"{rows} rows for {n} sequences: without `starts` each has one")
+        if seqs is None and n > self.lens.numel():
+            raise ValueError(f"{n} sequences, the cache has {self.lens.numel()}")
+        return n
+
+    # -- pages --------------------------------------------------------------------------
+    def free(self, seqs, stream: int) -> None:
+        n = self._list("free", seqs, seqs)
+        _check(lib.xpkKvFree(self.handle, seqs.data_ptr(), n, stream), "xpkKvFree")
+
+    def fork(self, parents, children, stream: int) -> None:
+        n = self._list("fork", parents, children)
+        _check(lib.xpkKvFork(self.handle, parents.data_ptr(), children.data_ptr(), n, stream), "xpkKvFork")
+
+    def extend(self, seqs, tokens, stream: int) -> None:
+        n = self._list("extend", seqs, tokens)
+        _check(lib.xpkKvExtend(self.handle, seqs.data_ptr(), tokens.data_ptr(), n, stream), "xpkKvExtend")
+
+    def compact(self, stream: int) -> None:
+        _check(lib.xpkKvCompact(self.handle, stream), "xpkKvCompact")
+
+    def copy(self, src, dst, stream: int) -> None:
+        n = self._list("copy", src, dst)
+        _check(lib.xpkKvCopy(self.handle, src.data_ptr(), dst.data_ptr(), n, stream), "xpkKvCopy")
+
+    def result(self, stream: int) -> KvReport:
+        """What the last extend or compact on the cache found (waits for the stream)."""
+        r = KvReport()
+        _check(lib.xpkKvResult(self.handle, C.byref(r), stream), "xpkKvResult")
+        return r
+
+    # -- new tokens ---------------------------------------------------------------------
+    def append(self, q, qkv, seqs, stream: int, *, starts=None, q_weight=None, k_weight=None, eps: float = 1e-6, inv_freq=None,
+               interleaved: bool = False, layer: int = 0) -> None:
+        """Norms, rotation and write of the rows of qkv [rows, (q_heads + 2 kv_heads) head_dim]; queries go to q [rows, q_heads, head_dim]."""
+        heads = q.numel() // max(1, q.shape[0] * self.dim)
+        rows, q_stride = _rows("q", q, heads * self.dim)
+        qkv_rows, qkv_stride = _rows("qkv", qkv, (heads + 2 * self.heads) * self.dim)
+        if rows != qkv_rows:
+            raise ValueError(f"{rows} rows of q, {qkv_rows} of qkv")
+        for name, w in (("q_weight", q_weight), ("k_weight", k_weight)):
+            if w is not None and (w.numel() != self.dim or not w.is_contiguous()):
+                raise ValueError(f"{name} has {self.dim} elements")
+        if inv_freq is not None and (str(inv_freq.dtype) != "torch.float64" or not inv_freq.is_contiguous() or inv_freq.device != self.device):
+            raise ValueError("inv_freq is a contiguous float64 tensor on the cache's device")
+        a = KvAppendArgs(self._data("q", q), self._data("qkv", qkv), q_stride, qkv_stride, self._ints("seqs", seqs), self._ints("starts", starts),
+                         self._data("q_weight", q_weight), self._data("k_weight", k_weight), None if inv_freq is None else inv_freq.data_ptr(), eps,
+                         self._entries(seqs, starts, rows), rows, heads, layer, 0 if inv_freq is None else 2 * inv_freq.numel(), interleaved)
+        _check(lib.xpkKvAppend(self.handle, C.byref(a), stream), "xpkKvAppend")
+
+    # -- attention ----------------------------------------------------------------------
+    def attention_scratch_bytes(self, rows: int, n: int, q_heads: int) -> int:
+        return int(lib.xpkAttentionScratchBytes(self.handle, rows, n, q_heads))
+
+    def _attention_args(self, out, q, seqs, starts, shared_len, scratch, layer, scale) -> AttentionArgs:
+        heads = q.numel() // max(1, q.shape[0] * self.dim)
+        rows, q_stride = _rows("q", q, heads * self.dim)
+        out_rows, out_stride = _rows("out", out, heads * self.dim)
+        if rows != out_rows:
+            raise ValueError(f"{rows} rows of q, {out_rows} of out")
+        if scratch.device != self.device or not scratch.is_contiguous():
+            raise ValueError("scratch is contiguous and on the cache's device")
+        return AttentionArgs(self._data("out", out), self._data("q", q), out_stride, q_stride, self._ints("seqs", seqs), self._ints("starts", starts),
+                             self._ints("shared_len", shared_len), scratch.data_ptr(), scratch.numel() * scratch.element_size(),
+                             self.dim ** -0.5 if scale is None else scale, self._entries(seqs, starts, rows), rows, heads, layer)
+
+    def attention(self, out, q, seqs, stream: int, *, scratch, starts=None, shared_len=None, layer: int = 0, scale: float | None = None) -> None:
+        """out = attention of q [rows, q_heads, head_dim] to the positions of its sequences; scale None: head_dim ** -0.5."""
+        a = self._attention_args(out, q, seqs, starts, shared_len, scratch, layer, scale)
+        _check(lib.xpkAttention(self.handle, C.byref(a), stream), "xpkAttention")
