@@ -313,7 +313,8 @@ def _check(kv, c, q, out, seqs, starts, scale=None, layer=0):
     mine = ~want[:, 0, 0].isnan()
     assert bool((out[~mine] == 7).all()), "rows of no sequence were written"
     off = ((out.double() - want).abs() / bound)[mine]
-    assert not bool(off.isnan().any()) and (off.numel() == 0 or float(off.max()) <= 1.0), float(off.max())
+    worst = float(off.max()) if off.numel() else 0.0                          # NaN stays NaN and fails
+    assert worst <= 1.0
 
 
 SHAPES = [("bf16", 32, 8, 128, 64), ("fp16", 7, 1, 64, 16), ("bf16", 6, 2, 64, 128), ("fp16", 8, 8, 128, 32), ("bf16", 20, 1, 128, 16), ("fp16", 64, 2, 64, 16)]
@@ -371,6 +372,7 @@ def test_shared_prefix(pk, kv, dtype, Hq, H, D, page, shared, counts, lens):
 def test_padding_repeated_sequences_and_scratch_that_is_used_again(pk, kv):
     lens = [200, 40, 0, 333]
     c = _filled(pk, lens, 16, 2, 64, torch.bfloat16, extra=2)
+    _share(c, lens, 64)                                                   # what shared_len promises
     scratch = torch.zeros(c.attention_scratch_bytes(40, 9, 8), dtype=torch.uint8, device="cuda")
     for seqs, counts in (([3, -1, 0, 3, 9, 2], [1, 2, 3, 4, 1, 2]), ([1], [40]), ([0, 0, 0, 0, 1, 1, 3, 3, 5], [1] * 9), ([-1, -1], [2, 2])):
         starts = np.concatenate([[0], np.cumsum(counts)]).tolist()
