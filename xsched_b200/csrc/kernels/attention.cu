@@ -8,8 +8,8 @@
 //
 // Three kinds of tickets:
 //   tiles   (256 rows, key head, a run of 128-position tiles) by a whole CTA on the tensor pipe: the prefix, and sequences
-//           of more than 16 rows;
-//   units   (16 rows, key head, a run of 16-position blocks) by one warp: sequences of up to 16 rows;
+//           of more than 32 rows;
+//   units   (16 rows, key head, a run of 16-position blocks) by one warp: sequences of up to 32 rows;
 //   merges  a few output rows by one warp, where a row's result comes from several runs: their weighted sum.
 // The cut is a function of the lengths and the device's SM count alone, and a merge adds the runs in their order, so the
 // result does not depend on who computed what, or on preemption.  Merges are claimed when no tile and no unit is left and
@@ -36,58 +36,12 @@ __device__ __forceinline__ int claim(Ctl *ctl, const AttnShared *sh, int which, 
     return t < (unsigned long long)total ? (int)t : -1;
 }
 
-// Claims the CTA's next tile item; every thread of the CTA comes here.
-template <bool kPreemptible>
-__device__ __forceinline__ int next_item(Ctl *ctl, AttnShared *sh) {
-    if (threadIdx.x == 0) {
-        sh->ticket = claim<kPreemptible>(ctl, sh, kTileTickets, sh->tiles);
-        sh->odd = 0;
-    }
-    __syncthreads();
-    return sh->ticket;
-}
-
-template <class T, int kDim, bool kPreemptible>
-__device__ __forceinline__ unsigned long long work_on_tiles(Ctl *ctl, const CUtensorMap *map_k, const CUtensorMap *map_v, const CacheView &c,
-                                                            const AttnArgs &a, AttnShared *sh, unsigned char *smem, Ring &ring, TileState &st) {
-    unsigned long long done = 0;
-    while (true) {
-        const int ticket = next_item<kPreemptible>(ctl, sh);
-        if (ticket < 0) return done;
-        const TileItem x = tile_ticket(a, c, sh, ticket);
-        work_tiles<T, kDim>(c, a, sh, ctl, smem, smem + 2 * tile_bytes<kDim>(), st, x);
-        tc_fence_before();
-        __syncthreads();
-        tc_fence_after();
-        if (sh->odd != 0u) {
-            if (sh->abort == 0u) redo_item<T, kDim>(c, a, map_k, map_v, sh, ctl, ring, x);
-            __syncthreads();
-        }
-        if (threadIdx.x == 0) {
-            if (x.slot0 >= 0) {
-                __threadfence();
-                atomicAdd(&a.counters[(size_t)(x.entry < 0 ? (int)a.n : x.entry) * c.heads + x.head], (uint32_t)(x.groups * x.half));
-            }
-            ++done;
-        }
-    }
-}
-
-template <class T, int kDim, bool kPreemptible>
-__device__ __forceinline__ void help_on_tiles(Ctl *ctl, const CUtensorMap *page_k, const CUtensorMap *page_v, const CacheView &c, const AttnArgs &a,
-                                              AttnShared *sh, unsigned char *smem, TileState &st) {
-    while (true) {
-        const int ticket = next_item<kPreemptible>(ctl, sh);
-        if (ticket < 0) return;
-        const TileItem x = tile_ticket(a, c, sh, ticket);
-        if (threadIdx.x == kWorkers * 32) load_tiles<kDim>(c, a, page_k, page_v, sh, ctl, smem + 2 * tile_bytes<kDim>(), st, x);
-        else if (threadIdx.x == kWorkers * 32 + 32) issue_tiles<T, kDim>(sh, ctl, smem, smem + 2 * tile_bytes<kDim>(), st, x);
-        __syncwarp();
-        tc_fence_before();
-        __syncthreads();
-        tc_fence_after();
-        if (sh->odd != 0u) __syncthreads();
-    }
+// An item from the loader; all lanes of a warp, or the issuing thread alone.
+__device__ __forceinline__ int next_item(AttnShared *sh, Ctl *ctl, uint32_t &seen) {
+    const uint32_t slot = seen % kSched;
+    if (!wait_bar(&sh->item_full[slot], (seen / kSched) & 1u, sh, ctl, kErrAttnTile)) return -1;
+    ++seen;
+    return *(volatile int *)&sh->item[slot];
 }
 
 // Some CTAs begin with tiles (tensor pipe), the others with units (HBM), so that both are busy; each goes on with the rest.
@@ -96,22 +50,41 @@ __device__ __forceinline__ void workers(Ctl *ctl, const CUtensorMap *map_k, cons
                                         AttnShared *sh, unsigned char *smem) {
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const bool tiles = sh->tiles > 0, tiles_first = (int)blockIdx.x < sh->tile_ctas;
-    Ring ring{smem + (size_t)warp * kUnitStages * unit_stage_bytes<kDim>(), sh->full[warp], 0u, 0u};
-    TileState st = {};
+    unsigned char *const unit_ring = smem + (size_t)warp * kUnitStages * unit_stage_bytes<kDim>();
+    Ring ring{unit_ring, sh->full[warp], kUnitStages, 0u, 0u, 0u, 0u};
     unsigned long long done = 0;
-    if (tiles && tiles_first) done += work_on_tiles<T, kDim, kPreemptible>(ctl, map_k, map_v, c, a, sh, smem, ring, st);
-    if (sh->units > 0)
-        while (true) {
-            int ticket = -1;
-            if (lane == 0) ticket = claim<kPreemptible>(ctl, sh, kUnitTickets, sh->units);
-            ticket = __shfl_sync(0xffffffffu, ticket, 0);
-            if (ticket < 0) break;
-            unit_ticket<T, kDim>(c, a, map_k, map_v, sh, ctl, ring, ticket);
-            done += lane == 0;
+    for (int phase = 0; phase < 2; ++phase) {
+        if ((phase == 0) != tiles_first) {
+            if (sh->units > 0)
+                while (true) {
+                    int ticket = -1;
+                    if (lane == 0) ticket = claim<kPreemptible>(ctl, sh, kUnitTickets, sh->units);
+                    ticket = __shfl_sync(0xffffffffu, ticket, 0);
+                    if (ticket < 0) break;
+                    unit_ticket<T, kDim>(c, a, map_k, map_v, sh, ctl, ring, ticket);
+                    done += lane == 0;
+                }
+            if (tiles && !tiles_first) __syncthreads();      // the units' rings lie where the tiles will: the loader waits here too
+        } else if (tiles) {
+            WorkState st = {};
+            uint32_t seen = 0;
+            while (true) {
+                const uint32_t slot = seen % kSched;
+                const int ticket = __shfl_sync(0xffffffffu, next_item(sh, ctl, seen), 0);
+                if (ticket < 0) break;
+                const TileItem x = tile_ticket(a, c, sh, ticket);
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&sh->item_empty[slot]);
+                work_tiles<T, kDim>(c, a, map_k, map_v, sh, ctl, smem, smem + 2 * query_bytes<kDim>(), st, ring, x);
+                done += threadIdx.x == 0;
+            }
+            // Both groups are through with the tiles' memory before units use it.
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&sh->worker_bar);
+            wait_bar(&sh->worker_bar, 0u, sh, ctl, kErrAttnTile);
+            __syncwarp();
+            ring.move(unit_ring, kUnitStages);
         }
-    if (tiles && !tiles_first) {
-        __syncthreads();                                    // the units' rings lie where the tiles will
-        done += work_on_tiles<T, kDim, kPreemptible>(ctl, map_k, map_v, c, a, sh, smem, ring, st);
     }
     // Without anything to do there is one merge of nothing, so that the call has a ticket to complete.
     while (true) {
@@ -123,8 +96,10 @@ __device__ __forceinline__ void workers(Ctl *ctl, const CUtensorMap *map_k, cons
         done += lane == 0;
     }
     // Loads that a unit gave up on still reach this CTA's shared memory: wait for them.
-    for (; ring.used != ring.loaded; ++ring.used)
-        wait_bar(&ring.full[ring.used % kUnitStages], (ring.used / kUnitStages) & 1u, sh, ctl, kErrAttnLoad, false);
+    while (ring.pending > 0) {
+        wait_bar(&ring.full[ring.using_], ring.parity(), sh, ctl, kErrAttnLoad, false);
+        ring.give();
+    }
     if (done) atomicAdd(&sh->done, done);
 }
 
@@ -132,15 +107,55 @@ template <class T, int kDim, bool kPreemptible>
 __device__ __forceinline__ void helpers(Ctl *ctl, const CUtensorMap *page_k, const CUtensorMap *page_v, const CacheView &c, const AttnArgs &a,
                                         AttnShared *sh, unsigned char *smem) {
     if (sh->tiles == 0) return;
-    TileState st = {};
     if ((int)blockIdx.x >= sh->tile_ctas) __syncthreads();
-    help_on_tiles<T, kDim, kPreemptible>(ctl, page_k, page_v, c, a, sh, smem, st);
-    // Loads and MMAs that were given up on: wait for them before the memories go.
-    if (threadIdx.x == kWorkers * 32) {
-        for (uint32_t s = st.stage > (uint32_t)kRing ? st.stage - kRing : 0u; s < st.stage; ++s)
+    unsigned char *tiles = smem + 2 * query_bytes<kDim>();
+    const int warp = __shfl_sync(0xffffffffu, (int)threadIdx.x >> 5, 0);
+    if (warp == kWorkers) {                                  // loader
+        const int lane = threadIdx.x & 31;
+        uint32_t stage = 0, given = 0, keys0 = 0, keys1 = 0, ends = 0;
+        while (true) {
+            int ticket = -1;
+            if (lane == 0) ticket = claim<kPreemptible>(ctl, sh, kTileTickets, sh->tiles);
+            ticket = __shfl_sync(0xffffffffu, ticket, 0);
+            const uint32_t slot = given % kSched;
+            if (!__all_sync(0xffffffffu, wait_bar(&sh->item_empty[slot], ((given / kSched) & 1u) ^ 1u, sh, ctl, kErrAttnTile))) break;
+            if (lane == 0) {
+                *(volatile int *)&sh->item[slot] = ticket;
+                mbar_arrive(&sh->item_full[slot]);
+            }
+            ++given;
+            if (ticket < 0) break;
+            const TileItem x = tile_ticket(a, c, sh, ticket);
+            if (!load_steps<kDim>(c, a, page_k, page_v, sh, ctl, tiles, stage, keys0, keys1, x)) break;
+            // Ahead into the next item only while every CTA still gets one: the last ones go to whoever is through.
+            bool ok = true;
+            for (int w = 0; w < 2; ++w) {
+                if ((w == 0 ? x.steps0 : x.steps1) == 0) continue;
+                if (ticket + (int)gridDim.x >= sh->tiles)
+                    ok = ok && __all_sync(0xffffffffu, wait_bar(&sh->o_full[w], ends >> w & 1u, sh, ctl, kErrAttnTile));
+                ends ^= 1u << w;
+            }
+            if (!ok) break;
+        }
+        // Loads that nobody waited for: before the memory goes.
+        for (uint32_t s = stage > (uint32_t)kRing ? stage - kRing : 0u; s < stage; ++s)
             wait_bar(&sh->ring_full[s % kRing], (s / kRing) & 1u, sh, ctl, kErrAttnTile, false);
-    } else if (threadIdx.x == kWorkers * 32 + 32) {
-        attn_commit(&sh->drain);
+    } else if (warp == kWorkers + 1) {                       // issuer
+        const uint32_t lead = elect_lead();
+        IssueState st = {};
+        uint32_t seen = 0;
+        while (true) {
+            const uint32_t slot = seen % kSched;
+            const int ticket = __shfl_sync(0xffffffffu, next_item(sh, ctl, seen), 0);
+            if (ticket < 0) break;
+            const TileItem x = tile_ticket(a, c, sh, ticket);
+            __syncwarp();
+            if (lead) mbar_arrive(&sh->item_empty[slot]);
+            const int n0 = __shfl_sync(0xffffffffu, x.steps0, 0), n1 = __shfl_sync(0xffffffffu, x.steps1, 0);
+            const bool both = __shfl_sync(0xffffffffu, (int)x.both, 0) != 0;
+            if (!issue_steps<T, kDim>(sh, ctl, smem, tiles, st, n0, n1, both, lead)) break;
+        }
+        attn_commit(&sh->drain, lead);
         wait_bar(&sh->drain, 0u, sh, ctl, kErrAttnTile, false);
     }
     __syncwarp();
@@ -151,12 +166,12 @@ __device__ __forceinline__ void work_off(Ctl *ctl, const CUtensorMap *map_k, con
                                          const CacheView &c, const AttnArgs &a, AttnShared *sh, unsigned char *smem) {
     const int warp = threadIdx.x >> 5;
     make_plan(c, a, sh);
+    const int merges = max(sh->merges, sh->tiles + sh->units == 0 ? 1 : 0);
+    const bool tiles = sh->tiles > 0;
     if (threadIdx.x == 0) {
         // Never zero: a task that was stopped before any CTA got here must not look complete.
-        if (sh->tiles + sh->units + sh->merges == 0) sh->merges = 1;
-        *(volatile unsigned long long *)&ctl->total = (unsigned long long)sh->tiles + sh->units + sh->merges;       // the same from every CTA
+        *(volatile unsigned long long *)&ctl->total = (unsigned long long)sh->tiles + sh->units + merges;       // the same from every CTA
     }
-    const bool tiles = sh->tiles > 0;
     if (tiles && warp == kWorkers + 1) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" :: "r"(smem_u32(&sh->tmem)), "r"(kAttnTmemCols) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
@@ -164,6 +179,7 @@ __device__ __forceinline__ void work_off(Ctl *ctl, const CUtensorMap *map_k, con
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
+    if (threadIdx.x == 0) sh->merges = merges;
     if (warp < kWorkers) {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" :: "n"(kWorkerRegs));
         workers<T, kDim, kPreemptible>(ctl, map_k, map_v, c, a, sh, smem);
@@ -191,7 +207,17 @@ attention_kernel(Ctl *ctl, const __grid_constant__ CUtensorMap map_k, const __gr
         for (int w = 0; w < kWorkers; ++w)
             for (int s = 0; s < kUnitStages; ++s) mbar_init(&sh->full[w][s], 1);
         for (int s = 0; s < kRing; ++s) { mbar_init(&sh->ring_full[s], 1); mbar_init(&sh->ring_empty[s], 1); }
-        for (int w = 0; w < 2; ++w) { mbar_init(&sh->q_full[w], 4); mbar_init(&sh->s_full[w], 1); mbar_init(&sh->p_full[w], 4); mbar_init(&sh->o_full[w], 1); }
+        for (int s = 0; s < kSched; ++s) { mbar_init(&sh->item_full[s], 1); mbar_init(&sh->item_empty[s], 1 + kWorkers); }
+        for (int w = 0; w < 2; ++w) {
+            mbar_init(&sh->q_full[w], 4);
+            mbar_init(&sh->pv_done[w], 1);
+            mbar_init(&sh->o_full[w], 1);
+            for (int b = 0; b < 2; ++b) { mbar_init(&sh->s_full[w][b], 1); mbar_init(&sh->p_full[w][b], 4); }
+            sh->odd[w] = 0;
+        }
+        mbar_init(&sh->group_bar[0], 4);
+        mbar_init(&sh->group_bar[1], 4);
+        mbar_init(&sh->worker_bar, kWorkers);
         mbar_init(&sh->drain, 1);
         sh->done = 0;
         sh->abort = 0;
@@ -247,7 +273,7 @@ AttnScratch attention_scratch(const CacheView &c, uint32_t sms, uint32_t rows, u
     // slots a result, two halves).  With a prefix every sharing sequence leaves some: one per key head if it is of one row
     // group (all are where each has a single query of up to 16 heads), at most eight; the prefix itself 16 per item.
     const size_t group = q_heads / c.heads, most = std::min<size_t>(n, rows);
-    const size_t base = 4 * (size_t)sms * kWorkers + 64 * (size_t)sms;
+    const size_t base = 2 * (size_t)kUnitWaves * sms * kWorkers + 64 * (size_t)sms;
     const size_t own = c.heads * most * (rows <= n && group <= kUnitRows ? 1 : 8);
     const size_t pre_rows = std::min<size_t>((size_t)rows * group, most * kShareRows);
     const size_t pre = 16 * (c.heads * ((pre_rows + kItemRows - 1) / kItemRows) + 2 * (size_t)sms);

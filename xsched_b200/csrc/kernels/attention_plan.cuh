@@ -14,14 +14,20 @@ constexpr int kWorkerRegs = 208, kHelperRegs = 88;
 static_assert(2 * kWorkerRegs + kHelperRegs <= 3 * 168, "more registers than the launch has");
 constexpr int kBlock = 16;                                  // positions per block of a unit
 constexpr int kUnitRows = 16;                               // rows of a unit, and of a partial result
+constexpr int kUnitRowsMost = 32;                           // sequences of more rows go by tiles
 constexpr int kUnitStages = 3;
+constexpr int kUnitWaves = 4;                               // units that each warp gets where there is enough work
 constexpr int kTile = 128;                                  // positions per tile; rows per group of a tile item
 constexpr int kItemRows = 2 * kTile;
-constexpr int kRing = 4;                                    // stages of the tile ring; a stage holds a tile of keys or of values
+constexpr int kStep = 64;                                   // positions per product; tiles are counted in pairs of steps
+constexpr int kRing = 8;                                    // stages of the tile ring; a stage holds a step's keys or values
 constexpr int kMinRun = 4;                                  // blocks: a run shorter than 64 positions costs more to merge than it spreads
 constexpr int kMinTiles = 2;                                // tiles: one for each group of workers
 constexpr int kShareRows = 64;                              // sequences of more rows fill tiles by themselves
 constexpr int kMergeRowsMost = 32;
+constexpr int kPageWords = 16;                              // more than the steps that a ring holds
+constexpr int kSched = 2;                                   // items the loader may be ahead
+constexpr float kTileUs = 1.6f;                             // measured time of a tile of 256 rows at head_dim 128
 constexpr uint32_t kErrAttnLoad  = 0x70000001u;
 constexpr uint32_t kErrAttnMerge = 0x70000002u;
 constexpr uint32_t kErrAttnTile  = 0x70000003u;
@@ -51,14 +57,17 @@ struct AttnShared {
     int part0[XPK_ATTENTION_MAX_SEQS];                      // its first partial result, -1: written directly
     int pre0[XPK_ATTENTION_MAX_SEQS];                       // rows of sharing sequences before it
     uint32_t share[XPK_ATTENTION_MAX_SEQS / 32];            // which sequences share
+    unsigned long long sums[4];                             // blocks, tiles, sharing rows, sharing sequences
+    int4 warp_sums[kAttnThreads / 32];
+    uint32_t first_sharing;
     // tile pipeline
     unsigned long long ring_full[kRing], ring_empty[kRing];
-    unsigned long long q_full[2], s_full[2], p_full[2], o_full[2], drain;
-    int ticket;
-    uint32_t tmem, odd, stage_pages[kRing];
+    unsigned long long item_full[kSched], item_empty[kSched];
+    unsigned long long q_full[2], s_full[2][2], p_full[2][2], pv_done[2], o_full[2], group_bar[2], worker_bar, drain;
+    int item[kSched];                                       // tickets handed to issuer and workers; -1: no more
+    uint32_t tmem, odd[2], pages[2][kPageWords];            // pages of the last steps of each order of keys that are there (bits)
     // units
     unsigned long long full[kWorkers][kUnitStages];
-    unsigned long long red[kAttnThreads / 32];
     unsigned long long done;
     int run, tile_run;                                      // blocks (tiles) per run
     int units, tiles, merges, merge_rows;
@@ -68,9 +77,10 @@ struct AttnShared {
 };
 
 template <int kDim> __host__ __device__ constexpr uint32_t unit_stage_bytes() { return 2 * kBlock * kDim * 2; }
-template <int kDim> __host__ __device__ constexpr uint32_t tile_bytes() { return kTile * kDim * 2; }
+template <int kDim> __host__ __device__ constexpr uint32_t query_bytes() { return kTile * kDim * 2; }       // of a group of workers
+template <int kDim> __host__ __device__ constexpr uint32_t step_bytes() { return kStep * kDim * 2; }
 template <int kDim> __host__ __device__ constexpr size_t ring_bytes() {
-    const size_t tiles = (size_t)(2 + kRing) * tile_bytes<kDim>(), units = (size_t)kWorkers * kUnitStages * unit_stage_bytes<kDim>();
+    const size_t tiles = (size_t)2 * query_bytes<kDim>() + (size_t)kRing * step_bytes<kDim>(), units = (size_t)kWorkers * kUnitStages * unit_stage_bytes<kDim>();
     return tiles > units ? tiles : units;
 }
 template <int kDim> __host__ __device__ constexpr size_t attn_smem() { return 1024 + ring_bytes<kDim>() + sizeof(AttnShared); }
@@ -140,7 +150,7 @@ __device__ __forceinline__ bool shares(const AttnShared *sh, int i) { return sh-
 // First position that a sequence's own runs cover.
 __device__ __forceinline__ int own_from(const AttnShared *sh, int i) { return shares(sh, i) ? sh->shared : 0; }
 __device__ __forceinline__ long long rows_of(const SeqPlan &p, uint32_t group) { return (long long)p.t * group; }
-__device__ __forceinline__ bool by_tiles(const SeqPlan &p, uint32_t group) { return rows_of(p, group) > kUnitRows; }
+__device__ __forceinline__ bool by_tiles(const SeqPlan &p, uint32_t group) { return rows_of(p, group) > kUnitRowsMost; }
 __device__ __forceinline__ int row_groups(long long rows) { return (int)((rows + kUnitRows - 1) / kUnitRows); }
 __device__ __forceinline__ int row_tiles(long long rows) { return (int)((rows + kItemRows - 1) / kItemRows); }
 // With at most 128 rows the two groups of workers take half of a run's tiles each, and leave a result each.
@@ -156,22 +166,20 @@ __device__ __forceinline__ int runs_of(const AttnShared *sh, uint32_t group, int
 __device__ __forceinline__ int pre_runs(const AttnShared *sh) { return tile_runs(sh, sh->shared) * halves(sh->pre_rows); }
 
 // ---- the cut ----------------------------------------------------------------------------------------------------
-__device__ __forceinline__ unsigned long long block_sum(unsigned long long v, AttnShared *sh) {
+__device__ __forceinline__ unsigned long long warp_sum(unsigned long long v) {
 #pragma unroll
     for (int d = 16; d > 0; d >>= 1) v += __shfl_xor_sync(0xffffffffu, v, d);
-    __syncthreads();
-    if ((threadIdx.x & 31) == 0) sh->red[threadIdx.x >> 5] = v;
-    __syncthreads();
-    unsigned long long s = 0;
-    for (int w = 0; w < kAttnThreads / 32; ++w) s += sh->red[w];
-    return s;
+    return v;
 }
 
-// Every CTA works the same cut out of the same arrays.
+// Every CTA works the same cut out of the same arrays, a thread per sequence.
 __device__ __forceinline__ void make_plan(const CacheView &c, const AttnArgs &a, AttnShared *sh) {
-    const uint32_t tid = threadIdx.x;
+    const uint32_t tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    constexpr uint32_t kWarps = kAttnThreads / 32;
     int shared = a.shared_len ? max(*a.shared_len, 0) & ~(int)(c.page - 1) : 0;
-    unsigned long long sharing = 0;
+    if (tid < 4) sh->sums[tid] = 0;
+    if (tid == 4) sh->first_sharing = 0xffffffffu;
+    __syncthreads();
     for (uint32_t base = 0; base < a.n; base += kAttnThreads) {              // whole warps: ballots below
         const uint32_t i = base + tid;
         bool with = false;
@@ -186,105 +194,120 @@ __device__ __forceinline__ void make_plan(const CacheView &c, const AttnArgs &a,
             with = shared > 0 && p.seq >= 0 && rows_of(p, a.group) <= kShareRows && p.len - p.t >= shared;
         }
         const uint32_t bits = __ballot_sync(0xffffffffu, with);
-        if ((tid & 31) == 0 && i < XPK_ATTENTION_MAX_SEQS) sh->share[i >> 5] = bits;
-        sharing += with;
+        if (lane == 0 && i < XPK_ATTENTION_MAX_SEQS) {
+            sh->share[i >> 5] = bits;
+            if (bits != 0) {
+                atomicAdd(&sh->sums[3], (unsigned long long)__popc(bits));
+                atomicMin(&sh->first_sharing, i + __ffs(bits) - 1);
+            }
+        }
     }
-    sharing = block_sum(sharing, sh);
-    if (sharing < 2) shared = 0;
+    __syncthreads();
+    if (sh->sums[3] < 2) shared = 0;
     // A second round without the prefix if its results do not fit the scratch.
     for (int round = 0; round < 2; ++round) {
-        if (shared == 0)
-            for (uint32_t i = tid; i < XPK_ATTENTION_MAX_SEQS / 32; i += kAttnThreads) sh->share[i] = 0;
-        if (tid == 0) sh->shared = shared;
+        if (shared == 0 && tid < XPK_ATTENTION_MAX_SEQS / 32) sh->share[tid] = 0;
+        if (tid == 0) {
+            sh->shared = shared;
+            sh->shared_seq = shared > 0 ? sh->plan[sh->first_sharing].seq : -1;
+        }
         __syncthreads();
         unsigned long long blocks = 0, tiles = 0, rows = 0;
         for (uint32_t i = tid; i < a.n; i += kAttnThreads) {
             const SeqPlan p = sh->plan[i];
             if (p.seq < 0) continue;
-            const int own = p.len - own_from(sh, i);
-            if (by_tiles(p, a.group)) tiles += (unsigned long long)((own + kTile - 1) / kTile) * row_tiles(rows_of(p, a.group)) * c.heads;
-            else blocks += (unsigned long long)((own + kBlock - 1) / kBlock) * c.heads;
-            if (shares(sh, i)) rows += (unsigned long long)rows_of(p, a.group);
+            const int own = p.len - own_from(sh, (int)i);
+            if (by_tiles(p, a.group)) tiles += (unsigned long long)((own + kTile - 1) / kTile) * row_tiles(rows_of(p, a.group));
+            else blocks += (unsigned long long)((own + kBlock - 1) / kBlock) * row_groups(rows_of(p, a.group));
+            if (shares(sh, (int)i)) rows += (unsigned long long)rows_of(p, a.group);
         }
-        blocks = block_sum(blocks, sh);
-        tiles = block_sum(tiles, sh);
-        rows = block_sum(rows, sh);
-        tiles += (unsigned long long)((shared + kTile - 1) / kTile) * row_tiles(rows) * c.heads;
+        if (warp * 32 < a.n) {
+            blocks = warp_sum(blocks);
+            tiles = warp_sum(tiles);
+            rows = warp_sum(rows);
+            if (lane == 0) {
+                atomicAdd(&sh->sums[0], blocks);
+                atomicAdd(&sh->sums[1], tiles);
+                atomicAdd(&sh->sums[2], rows);
+            }
+        }
+        __syncthreads();
+        blocks = sh->sums[0] * c.heads;
+        rows = sh->sums[2];
+        tiles = (sh->sums[1] + (unsigned long long)((shared + kTile - 1) / kTile) * row_tiles((long long)rows)) * c.heads;
+        const unsigned long long target = (unsigned long long)a.sms * kWorkers * kUnitWaves;
         if (tid == 0) {
-            const unsigned long long target = (unsigned long long)a.sms * kWorkers * 2;
             sh->run = max(kMinRun, (int)min((blocks + target - 1) / target, 0x7fffffffull / kBlock));
             sh->tile_run = max(kMinTiles, (int)min((tiles + a.sms - 1) / a.sms, 0x7fffffffull / kTile));
             sh->pre_rows = (int)rows;
-            // CTAs are dealt to tiles and units by the time each kind takes: a tile of 256 rows about 1.3 us of an SM, a block
+            // CTAs are dealt to tiles and units by the time each kind takes: a tile of 256 rows about kTileUs of an SM, a block
             // 64 bytes an element over the SM's share of HBM (44 GB/s): 0.19 us at 128.
-            const float tile_us = 1.3f * (float)tiles, block_us = 0.0015f * (float)c.dim * (float)blocks;
+            const float tile_us = kTileUs * (float)tiles * ((float)c.dim / 128.f), block_us = 0.0015f * (float)c.dim * (float)blocks;
             sh->tile_ctas = tiles == 0 ? 0 : blocks == 0 ? 0x7fffffff : max(1, (int)((float)gridDim.x * tile_us / (tile_us + block_us) + 0.5f));
         }
         __syncthreads();
-        // Tickets and partial results before each sequence: a running sum, 32 sequences at a time, by the first warp.
-        if (tid < 32) {
-            int units = 0, items = 0, parts = 0, pre = 0;
-            if (shared > 0) items = row_tiles(sh->pre_rows) * (int)c.heads * tile_runs(sh, shared);
-            const int pre_items = items;
-            for (uint32_t base = 0; base < a.n; base += 32) {
-                const uint32_t i = base + tid;
-                int u = 0, x = 0, r = 0, s = 0;
-                if (i < a.n && sh->plan[i].seq >= 0) {
-                    const SeqPlan p = sh->plan[i];
-                    const long long rs = rows_of(p, a.group);
-                    const int runs = runs_of(sh, a.group, (int)i);
-                    if (by_tiles(p, a.group)) x = row_tiles(rs) * (int)c.heads * (runs / halves(rs));
-                    else u = (int)c.heads * runs;
-                    if (runs > 1 || shares(sh, (int)i)) r = row_groups(rs) * (int)c.heads * runs;
-                    if (shares(sh, (int)i)) s = (int)rs;
-                }
-                int us = u, xs = x, rsum = r, ss = s;
+        // Tickets and partial results before each sequence: a scan in each warp, then over the warps.
+        int4 carry = make_int4(0, 0, 0, 0);
+        if (shared > 0) carry.y = row_tiles(sh->pre_rows) * (int)c.heads * tile_runs(sh, shared);
+        const int pre_items = carry.y;
+        for (uint32_t base = 0; base < a.n; base += kAttnThreads) {
+            const uint32_t i = base + tid;
+            int4 v = make_int4(0, 0, 0, 0);                                  // units, tile items, results, sharing rows
+            if (i < a.n && sh->plan[i].seq >= 0) {
+                const SeqPlan p = sh->plan[i];
+                const long long rs = rows_of(p, a.group);
+                const int runs = runs_of(sh, a.group, (int)i), groups = row_groups(rs) * (int)c.heads;
+                if (by_tiles(p, a.group)) v.y = row_tiles(rs) * (int)c.heads * (runs / halves(rs));
+                else v.x = groups * runs;
+                if (runs > 1 || shares(sh, (int)i)) v.z = groups * runs;
+                if (shares(sh, (int)i)) v.w = (int)rs;
+            }
+            int4 s = v;
+            if (base + warp * 32 < a.n) {
 #pragma unroll
                 for (int d = 1; d < 32; d <<= 1) {
-                    const int y0 = __shfl_up_sync(0xffffffffu, us, d), y1 = __shfl_up_sync(0xffffffffu, xs, d);
-                    const int y2 = __shfl_up_sync(0xffffffffu, rsum, d), y3 = __shfl_up_sync(0xffffffffu, ss, d);
-                    if ((int)tid >= d) { us += y0; xs += y1; rsum += y2; ss += y3; }
+                    const int y0 = __shfl_up_sync(0xffffffffu, s.x, d), y1 = __shfl_up_sync(0xffffffffu, s.y, d);
+                    const int y2 = __shfl_up_sync(0xffffffffu, s.z, d), y3 = __shfl_up_sync(0xffffffffu, s.w, d);
+                    if ((int)lane >= d) { s.x += y0; s.y += y1; s.z += y2; s.w += y3; }
                 }
-                if (i < a.n) {
-                    sh->unit0[i] = units + us - u;
-                    sh->tile0[i] = items + xs - x;
-                    sh->part0[i] = r > 0 ? parts + rsum - r : -1;
-                    sh->pre0[i] = pre + ss - s;
-                }
-                units += __shfl_sync(0xffffffffu, us, 31);
-                items += __shfl_sync(0xffffffffu, xs, 31);
-                parts += __shfl_sync(0xffffffffu, rsum, 31);
-                pre += __shfl_sync(0xffffffffu, ss, 31);
             }
-            if (tid == 0) {
-                sh->units = units;
-                sh->tiles = items;
-                sh->pre_tiles = pre_items;
-                sh->pre_part0 = parts;
-                if (shared > 0) parts += row_groups(sh->pre_rows) * (int)c.heads * pre_runs(sh);
-                sh->last = parts > (int)a.part_slots;          // borrowed as a flag until the end of the kernel
-                const uint32_t out_rows = a.rows * a.q_heads;
-                int per = 1;
-                while (per < kMergeRowsMost && (unsigned long long)per * a.sms * kWorkers < out_rows) per *= 2;
-                sh->merge_rows = per;
-                sh->merges = parts > 0 ? (int)((out_rows + per - 1) / per) : 0;
+            if (lane == 31) sh->warp_sums[warp] = s;
+            __syncthreads();
+            int4 before = carry;
+            for (uint32_t w = 0; w < kWarps && base + w * 32 < a.n; ++w) {
+                const int4 y = sh->warp_sums[w];
+                if (w < warp) { before.x += y.x; before.y += y.y; before.z += y.z; before.w += y.w; }
+                carry.x += y.x; carry.y += y.y; carry.z += y.z; carry.w += y.w;
             }
+            if (i < a.n) {
+                sh->unit0[i] = before.x + s.x - v.x;
+                sh->tile0[i] = before.y + s.y - v.y;
+                sh->part0[i] = v.z > 0 ? before.z + s.z - v.z : -1;
+                sh->pre0[i] = before.w + s.w - v.w;
+            }
+            __syncthreads();
         }
-        __syncthreads();
-        if (sh->last == 0u || shared == 0) break;
-        shared = 0;
-        __syncthreads();
-    }
-    if (sh->shared > 0) {                                       // the first sharing sequence's table names the prefix's pages
-        if (tid < 32) {
-            const uint32_t mine = tid < XPK_ATTENTION_MAX_SEQS / 32 && tid * 32 < a.n ? sh->share[tid] : 0u;
-            const uint32_t some = __ballot_sync(0xffffffffu, mine != 0u);
-            const int word = __ffs(some) - 1;
-            const uint32_t bits = __shfl_sync(0xffffffffu, mine, word);
-            if (tid == 0) sh->shared_seq = sh->plan[word * 32 + __ffs(bits) - 1].seq;
+        int parts = carry.z;
+        if (shared > 0) parts += row_groups(sh->pre_rows) * (int)c.heads * pre_runs(sh);
+        if (shared > 0 && parts > (int)a.part_slots) {                        // the same for all threads
+            shared = 0;
+            if (tid < 3) sh->sums[tid] = 0;
+            continue;
         }
-        __syncthreads();
+        if (tid == 0) {
+            sh->units = carry.x;
+            sh->tiles = carry.y;
+            sh->pre_tiles = pre_items;
+            sh->pre_part0 = carry.z;
+            const uint32_t out_rows = a.rows * a.q_heads;
+            int per = 1;
+            while (per < kMergeRowsMost && (unsigned long long)per * a.sms * kWorkers < out_rows) per *= 2;
+            sh->merge_rows = per;
+            sh->merges = parts > 0 ? (int)((out_rows + per - 1) / per) : 0;
+        }
+        break;
     }
+    __syncthreads();
 }
 
 // ---- waits -------------------------------------------------------------------------------------------------------

@@ -1,42 +1,51 @@
 // Tiles of an attention call (see attention.cu): up to 256 rows against 128 positions at a time on the tensor pipe.
 //
 // Two groups of four warps take 128 rows each (thread = row), or, where an item has at most 128 rows, the same rows and one
-// half of the positions each.  Per tile and group:
+// half of the positions each.  Per step of 64 positions and group:
 //
-//   S = Q K^T     tcgen05.mma M128 N128, Q and K from shared memory (K-major), S fp32 in tensor memory
+//   S = Q K^T     tcgen05.mma M128 N64, Q and K from shared memory (K-major), S fp32 in tensor memory, two buffers
 //   P = exp2(..)  the group's threads read their rows of S, keep maximum and sum, and write P (16 bit) over S
 //   O += P V      tcgen05.mma with P from tensor memory and V from shared memory (dimension-major: V lies as it is stored)
 //
-// One thread issues the MMAs of both groups in turn, so that one group's exponentials run under the other's products;
-// another fills a ring of four stages (a tile of K or of V, 32 KB) by TMA, page by page.  MMAs of one thread execute in the
-// order of issue: S of tile j + 1 may overwrite P of tile j once P V of tile j has been issued.  The barrier that says
-// "S is there" therefore also says that the P V before it is done, and the group may touch O.
+// One thread issues the MMAs of both groups in turn; S of step s + 2 follows P V of step s, so a group always finds its next
+// scores there while the pipe works for the other.  MMAs of one thread execute in the order of issue: that is what lets S of
+// step s + 2 overwrite P of step s.  Another thread claims the items and fills a ring of eight stages (a step of K or of V,
+// 16 KB each at 128) by TMA, page by page, and runs ahead of the rest into the next item.
 //
 // O is not rescaled whenever the maximum grows: p is taken relative to a reference that follows the maximum only when it
-// falls 2^8 behind, so p stays below 2^8 (fp16 holds 2^15) and almost every tile leaves O alone.
+// falls 2^8 behind, so p stays below 2^8 (fp16 holds 2^15) and almost every step leaves O alone.
 //
 // Bound by the tensor pipe (4 * 128 * 128 * head_dim flop per group and tile: 0.55 us at 128) and by the exponentials
 // (16 a clock and SM: 0.55 us) alike; K and V of a tile are fetched once for 256 rows.
 #pragma once
 #include "attention_units.cuh"
 
+#include <type_traits>
+
 namespace xpk {
 
 constexpr float kLag = 8.f;                                  // log2 units that the reference may fall behind the maximum
 
 // ---- instructions ------------------------------------------------------------------------------------------------
-__device__ __forceinline__ void attn_commit(void *bar) {
-    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" :: "r"(smem_u32(bar)) : "memory");
+// The issuing warp runs as one (its addresses and descriptors stay in uniform registers); `lead` is 1 in the one lane that issues.
+__device__ __forceinline__ uint32_t elect_lead() {
+    uint32_t lead;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(lead));
+    return lead;
 }
-__device__ __forceinline__ void attn_mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
-    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-                 "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
-                 :: "r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
+__device__ __forceinline__ void attn_commit(void *bar, uint32_t lead) {
+    asm volatile("{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %1, 0;\n\t"
+                 "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" :: "r"(smem_u32(bar)), "r"(lead) : "memory");
 }
-__device__ __forceinline__ void attn_mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
-    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-                 "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
-                 :: "r"(d), "r"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
+__device__ __forceinline__ void attn_mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate, uint32_t lead) {
+    asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %5, 0;\n\t"
+                 "@q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
+                 :: "r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate), "r"(lead) : "memory");
+}
+__device__ __forceinline__ void attn_mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate, uint32_t lead) {
+    asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %5, 0;\n\t"
+                 "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
+                 :: "r"(d), "r"(a), "l"(b), "r"(idesc), "r"(accumulate), "r"(lead) : "memory");
 }
 __device__ __forceinline__ void tc_st32(uint32_t taddr, const uint32_t *r) {
     asm volatile("tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], "
@@ -47,14 +56,23 @@ __device__ __forceinline__ void tc_st32(uint32_t taddr, const uint32_t *r) {
                     "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]),
                     "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31]), "r"(taddr) : "memory");
 }
+// Waits for loads from tensor memory.  The registers pass through an empty statement behind the wait: arithmetic on them has
+// no other reason to stay behind it.
+template <int N>
+__device__ __forceinline__ void tc_landed(uint32_t (&r)[N]) {
+    tc_wait_ld();
+#pragma unroll
+    for (int i = 0; i < N; i += 8)
+        asm volatile("" : "+r"(r[i]), "+r"(r[i + 1]), "+r"(r[i + 2]), "+r"(r[i + 3]), "+r"(r[i + 4]), "+r"(r[i + 5]), "+r"(r[i + 6]), "+r"(r[i + 7]));
+}
 __device__ __forceinline__ void tc_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
 // V as B operand with the dimension contiguous: atoms of 64 dimensions x 8 positions (1024 B, 128-byte swizzle), the next
-// eight positions behind it, the next 64 dimensions a whole tile of 128 positions further.
+// eight positions behind it, the next 64 dimensions a whole step of 64 positions further.
 __device__ __forceinline__ uint64_t make_v_desc(uint32_t smem_addr) {
     uint64_t d = 0;
     d |= (uint64_t)((smem_addr & 0x3FFFFu) >> 4);
-    d |= (uint64_t)((kTile * 128u) >> 4) << 16;              // leading byte offset: between blocks of 64 dimensions
+    d |= (uint64_t)((kStep * 128u) >> 4) << 16;              // leading byte offset: between blocks of 64 dimensions
     d |= (uint64_t)(1024u >> 4) << 32;                       // stride byte offset: between groups of eight positions
     d |= (uint64_t)1 << 46;
     d |= (uint64_t)2 << 61;
@@ -62,14 +80,14 @@ __device__ __forceinline__ uint64_t make_v_desc(uint32_t smem_addr) {
 }
 template <class T> __host__ __device__ constexpr uint32_t mma_type() { return sizeof(T) == 2 ? 1u : 0u; }
 template <> __host__ __device__ constexpr uint32_t mma_type<__half>() { return 0u; }
-// D fp32; N = 128 positions, both K-major; N = kDim, B with N contiguous.
+// D fp32, M = 128 rows; N = 64 positions, both K-major; N = kDim, B with N contiguous.
 template <class T> __host__ __device__ constexpr uint32_t idesc_s() {
-    return (1u << 4) | (mma_type<T>() << 7) | (mma_type<T>() << 10) | ((uint32_t)(kTile >> 3) << 17) | ((uint32_t)(kTile >> 4) << 24);
+    return (1u << 4) | (mma_type<T>() << 7) | (mma_type<T>() << 10) | ((uint32_t)(kStep >> 3) << 17) | ((uint32_t)(kTile >> 4) << 24);
 }
 template <class T, int kDim> __host__ __device__ constexpr uint32_t idesc_o() {
     return (1u << 4) | (mma_type<T>() << 7) | (mma_type<T>() << 10) | (1u << 16) | ((uint32_t)(kDim >> 3) << 17) | ((uint32_t)(kTile >> 4) << 24);
 }
-constexpr uint32_t kAttnTmemCols = 512;                      // S of both groups (128 each), O of both (head_dim each)
+constexpr uint32_t kAttnTmemCols = 512;                      // two S of both groups (64 columns each), O of both (head_dim each)
 
 // ---- an item -----------------------------------------------------------------------------------------------------
 struct TileItem {
@@ -78,7 +96,8 @@ struct TileItem {
     int from, end;              // positions [from, end) are the item's
     int seq;                    // whose table names the pages
     bool both;                  // both groups take every tile
-    int first[2], count[2];     // tiles of each group, counted from `from`
+    int pos0, pos1;             // where the two groups begin
+    int steps0, steps1;         // and how many steps of 64 positions they take
     int groups, half;           // groups of 16 rows; results per row of one run (2: one from each group of workers)
     int slot0, step;            // partial results: slot0 + group of 16 rows * step (+ half); slot0 < 0: the output itself
 };
@@ -123,179 +142,207 @@ __device__ __forceinline__ TileItem tile_ticket(const AttnArgs &a, const CacheVi
     }
     const int first = run * sh->tile_run, last = min(first + sh->tile_run, (most + kTile - 1) / kTile), count = max(last - first, 0);
     x.both = x.half == 1 && x.rows > kTile;
-    x.first[0] = x.first[1] = first;
-    x.count[0] = x.count[1] = count;
-    if (x.half == 2) {
-        x.count[0] = (count + 1) / 2;
-        x.first[1] = first + x.count[0];
-        x.count[1] = count - x.count[0];
-    } else if (!x.both) {
-        x.count[1] = 0;
-    }
+    const int head_tiles = x.half == 2 ? (count + 1) / 2 : count;              // of the first group where each takes a half
+    x.pos0 = x.from + first * kTile;
+    x.pos1 = x.half == 2 ? x.pos0 + head_tiles * kTile : x.pos0;
+    const int left = x.from + min(most, last * kTile);                          // nothing behind it is seen
+    x.steps0 = max(0, min(2 * head_tiles, (left - x.pos0 + kStep - 1) / kStep));
+    x.steps1 = x.both ? x.steps0 : x.half == 2 ? max(0, (left - x.pos1 + kStep - 1) / kStep) : 0;
     const int base = x.entry < 0 ? sh->pre_part0 : sh->part0[x.entry];
     x.step = runs * x.half;
     x.slot0 = base < 0 ? -1 : base + (x.head * row_groups(all) + x.r0 / kUnitRows) * x.step + run * x.half;
     return x;
 }
 
-// Counts of phases that each role has gone through; they go on from item to item.
-struct TileState {
-    uint32_t stage;             // ring stages filled (loader) or consumed (issuer, workers: in the order of loading)
-    uint32_t s, o;              // workers: tiles with scores and items with results of their group
-    uint32_t q[2], p[2];        // issuer: items with queries and tiles with weights of each group
-};
-
-// The order in which tiles of K and V are used: f(tile, is_v, group) for each stage of the ring.
+// The order in which steps of K and V are loaded and used: both groups' (or the common) first two K, then V of a step and K of
+// the step after next.  f(step, is_v, group).
 template <class F>
 __device__ __forceinline__ bool in_order(const TileItem &x, F f) {
-    if (x.both) {
-        const int n = x.count[0];
-        if (n > 0 && !f(x.first[0], false, 0)) return false;
-        for (int j = 0; j < n; ++j) {
-            if (!f(x.first[0] + j, true, 0)) return false;
-            if (j + 1 < n && !f(x.first[0] + j + 1, false, 0)) return false;
-        }
-        return true;
+    const int n0 = x.steps0, n1 = x.both ? 0 : x.steps1;
+    for (int s = 0; s < min(2, n0); ++s)
+        if (!f(s, false, 0)) return false;
+    for (int s = 0; s < min(2, n1); ++s)
+        if (!f(s, false, 1)) return false;
+    for (int s = 0; s < max(n0, n1); ++s) {
+        if (s < n0 && !f(s, true, 0)) return false;
+        if (s + 2 < n0 && !f(s + 2, false, 0)) return false;
+        if (s < n1 && !f(s, true, 1)) return false;
+        if (s + 2 < n1 && !f(s + 2, false, 1)) return false;
     }
-    for (int w = 0; w < 2; ++w)
-        if (x.count[w] > 0 && !f(x.first[w], false, w)) return false;
-    for (int j = 0; j < max(x.count[0], x.count[1]); ++j)
-        for (int w = 0; w < 2; ++w) {
-            if (j >= x.count[w]) continue;
-            if (!f(x.first[w] + j, true, w)) return false;
-            if (j + 1 < x.count[w] && !f(x.first[w] + j + 1, false, w)) return false;
-        }
     return true;
 }
+__device__ __forceinline__ uint32_t stages_of(const TileItem &x) { return 2u * (uint32_t)(x.steps0 + (x.both ? 0 : x.steps1)); }
+// Where V of a group's step lies in that order.
+__device__ __forceinline__ uint32_t v_stage(const TileItem &x, int w, int s) {
+    const int n0 = x.steps0, n1 = x.both ? 0 : x.steps1, before0 = w == 0 || x.both ? s : s + 1, before1 = s;
+    return (uint32_t)(min(2, n0) + min(2, n1) + min(before0, n0) + min(before0, max(n0 - 2, 0)) + min(before1, n1) + min(before1, max(n1 - 2, 0)));
+}
 
-// ---- loader (one thread) -----------------------------------------------------------------------------------------
+// ---- loader (one warp) -------------------------------------------------------------------------------------------
+// The ids of 32 pages of an order of steps, one per lane (-1: not there); `base`: the first one, counted from the order's first page.
+struct PageWindow {
+    int base, id;
+    uint32_t there;             // bit l: lane l's page is there
+};
+
+// A stage costs the loading warp about forty instructions: a thread by itself, looking pages up one by one, was what bounded a step
+// (0.5 us a stage).  Lanes hold page ids ahead and each issues one box.
 template <int kDim>
-__device__ __forceinline__ void load_tiles(const CacheView &c, const AttnArgs &a, const CUtensorMap *map_k, const CUtensorMap *map_v, AttnShared *sh,
-                                           Ctl *ctl, unsigned char *ring, TileState &st, const TileItem &x) {
+__device__ __forceinline__ bool load_steps(const CacheView &c, const AttnArgs &a, const CUtensorMap *map_k, const CUtensorMap *map_v, AttnShared *sh,
+                                           Ctl *ctl, unsigned char *ring, uint32_t &stage, uint32_t &keys0, uint32_t &keys1, const TileItem &x) {
+    constexpr int kHalves = kDim / 64;
+    const int lane = threadIdx.x & 31, shift = (int)c.page_shift;
     const int32_t *row = c.table + (size_t)x.seq * c.width;
-    const int per = kTile >> c.page_shift;                     // pages of a tile
-    in_order(x, [&](int tile, bool is_v, int) {
-        const uint32_t s = st.stage % kRing;
-        if (!wait_bar(&sh->ring_empty[s], ((st.stage / kRing) & 1u) ^ 1u, sh, ctl, kErrAttnTile)) return false;
-        unsigned char *dst = ring + (size_t)s * tile_bytes<kDim>();
-        const int pos = x.from + tile * kTile;
-        uint32_t there = 0;
-        int ids[kTile / 16];
-#pragma unroll
-        for (int j = 0; j < kTile / 16; ++j) {
-            if (j >= per) break;
-            const int at = pos + (j << c.page_shift);
-            int id = at < x.end ? row[at >> c.page_shift] : -1;
-            if (id < 0 || (uint32_t)id >= c.pages) id = -1; else there |= 1u << j;
-            ids[j] = id;
+    const int boxes = max(1, kStep >> shift);                 // pages of a step; a page of 128 holds two steps
+    const int mine = lane / kHalves, half = lane % kHalves;   // page and half of this lane's box
+    auto window = [&](int first, int pos0) {
+        PageWindow p;
+        p.base = first;
+        const long long at = (long long)((pos0 >> shift) + first + lane) << shift;
+        p.id = at < x.end ? row[at >> shift] : -1;
+        if (p.id < 0 || (uint32_t)p.id >= c.pages) p.id = -1;
+        p.there = __ballot_sync(0xffffffffu, p.id >= 0);
+        return p;
+    };
+    PageWindow win[2] = {window(0, x.pos0), {0, -1, 0u}};
+    if (!x.both && x.steps1 > 0) win[1] = window(0, x.pos1);
+    return in_order(x, [&](int step, bool is_v, int w) {
+        const int pos0 = w == 0 ? x.pos0 : x.pos1, pos = pos0 + step * kStep;
+        PageWindow &p = win[w];
+        const int first = (pos >> shift) - (pos0 >> shift);
+        // Keys run ahead of values by two steps: the window moves with them and keeps what the values still need.
+        if (first + boxes > p.base + 32) p = window(((pos0 + max(step - 2, 0) * kStep) >> shift) - (pos0 >> shift), pos0);
+        const uint32_t s = stage % kRing;
+        if (!__all_sync(0xffffffffu, wait_bar(&sh->ring_empty[s], ((stage / kRing) & 1u) ^ 1u, sh, ctl, kErrAttnTile))) return false;
+        const int id = __shfl_sync(0xffffffffu, p.id, first - p.base + min(mine, boxes - 1));
+        if (lane == 0) {
+            // The workers read the word of a step's keys once they have its scores; they are less than a ring behind.
+            if (!is_v) sh->pages[w][(w == 0 ? keys0 : keys1) % kPageWords] = p.there >> (first - p.base) & ((1u << boxes) - 1u);
+            mbar_arrive_expect_tx(&sh->ring_full[s], step_bytes<kDim>());
         }
-        sh->stage_pages[s] = there;                            // read by the workers once the stage is full
-        mbar_arrive_expect_tx(&sh->ring_full[s], tile_bytes<kDim>());
-#pragma unroll
-        for (int j = 0; j < kTile / 16; ++j) {
-            if (j >= per) break;
-            const int z = ids[j] < 0 ? -1 : (int)(a.layer * c.pages) + ids[j];        // outside the pool: zeros
-#pragma unroll
-            for (int h = 0; h < kDim / 64; ++h)
-                tma_load_3d(dst + h * (kTile * 128) + ((size_t)j << c.page_shift) * 128, is_v ? map_v : map_k, &sh->ring_full[s], h * 64,
-                            x.head * (int)c.page, z);
-        }
-        ++st.stage;
+        if (!is_v) { if (w == 0) ++keys0; else ++keys1; }
+        __syncwarp();
+        if (lane < boxes * kHalves)                            // a page that is not there: outside the pool, zeros
+            tma_load_3d(ring + (size_t)s * step_bytes<kDim>() + half * (kStep * 128) + ((size_t)mine << shift) * 128, is_v ? map_v : map_k,
+                        &sh->ring_full[s], half * 64, x.head * (int)c.page + (pos & (int)(c.page - 1)), id < 0 ? -1 : (int)(a.layer * c.pages) + id);
+        ++stage;
         return true;
     });
 }
 
-// ---- issuer (one thread) -----------------------------------------------------------------------------------------
+// ---- issuer (one warp) -------------------------------------------------------------------------------------------
+struct IssueState {
+    uint32_t stage;             // ring stages consumed, in the order of loading
+    uint32_t q, p;              // parities to wait for: queries (bit: group), weights (bit: 2 * group + buffer)
+};
+
+// A step is 2 * (8 + 4) MMAs, six commits and four waits at head_dim 128, and has to be issued in about 1300 clocks.  Groups and buffers
+// are unrolled, so descriptors are constants plus the stage's offset and parities are bits of one register.
 template <class T, int kDim>
-__device__ __forceinline__ void issue_tiles(AttnShared *sh, Ctl *ctl, unsigned char *smem_q, unsigned char *ring, TileState &st, const TileItem &x) {
-    const uint32_t tmem = *(volatile uint32_t *)&sh->tmem;
-    const uint32_t q0 = smem_u32(smem_q), r0 = smem_u32(ring);
-    auto full = [&](uint32_t stage) { return wait_bar(&sh->ring_full[stage % kRing], (stage / kRing) & 1u, sh, ctl, kErrAttnTile); };
-    auto scores = [&](int w, uint32_t stage) {                // S_w = Q_w K^T
-        const uint32_t q = q0 + w * tile_bytes<kDim>(), k = r0 + (stage % kRing) * tile_bytes<kDim>();
-#pragma unroll
-        for (int i = 0; i < kDim / 16; ++i) {
-            const uint32_t off = (i / 4) * (kTile * 128) + (i % 4) * 32;
-            attn_mma_ss(tmem + w * kTile, make_kmajor_sw128_desc(q + off), make_kmajor_sw128_desc(k + off), idesc_s<T>(), i > 0);
-        }
-        attn_commit(&sh->s_full[w]);
+__device__ __forceinline__ bool issue_steps(AttnShared *sh, Ctl *ctl, unsigned char *smem_q, unsigned char *ring, IssueState &st, int n0, int n1,
+                                            bool both, uint32_t lead) {
+    const uint32_t tmem = __shfl_sync(0xffffffffu, *(volatile uint32_t *)&sh->tmem, 0);
+    const uint64_t qd = make_kmajor_sw128_desc(smem_u32(smem_q)), kd = make_kmajor_sw128_desc(smem_u32(ring)), vd = make_v_desc(smem_u32(ring));
+    auto full = [&](uint32_t stage) {
+        const bool ok = __all_sync(0xffffffffu, wait_bar(&sh->ring_full[stage % kRing], (stage / kRing) & 1u, sh, ctl, kErrAttnTile));
+        tc_fence_after();
+        return ok;
     };
-    auto product = [&](int w, uint32_t stage, bool add) {     // O_w (+)= P_w V
-        const uint32_t v = r0 + (stage % kRing) * tile_bytes<kDim>();
+    auto scores = [&](int w, int b, uint32_t stage) {         // S_w = Q_w K^T, into buffer b
+        const uint64_t q = qd + (uint64_t)(w * (query_bytes<kDim>() >> 4)), k = kd + (uint64_t)((stage % kRing) * (step_bytes<kDim>() >> 4));
+        const uint32_t d = tmem + w * kTile + b * kStep;
 #pragma unroll
-        for (int i = 0; i < kTile / 16; ++i)
-            attn_mma_ts(tmem + 2 * kTile + w * kDim, tmem + w * kTile + i * 8, make_v_desc(v + i * 2048), idesc_o<T, kDim>(), add || i > 0);
+        for (int i = 0; i < kDim / 16; ++i)
+            attn_mma_ss(d, q + (uint64_t)((i / 4) * (kTile * 128 >> 4) + (i % 4) * 2), k + (uint64_t)((i / 4) * (kStep * 128 >> 4) + (i % 4) * 2),
+                        idesc_s<T>(), i > 0, lead);
+        attn_commit(&sh->s_full[w][b], lead);
     };
+    // O_w (+)= P_w V.  pv_done counts products: the group looks at it only for the newest or the one before, since a parity tells
+    // no more apart; the item's last one has a barrier of its own.
+    auto product = [&](int w, int b, uint32_t stage, bool first, bool last) {
+        const uint64_t v = vd + (uint64_t)((stage % kRing) * (step_bytes<kDim>() >> 4));
+        const uint32_t d = tmem + 2 * kTile + w * kDim, p = tmem + w * kTile + b * kStep;
+#pragma unroll
+        for (int i = 0; i < kStep / 16; ++i) attn_mma_ts(d, p + i * 8, v + (uint64_t)(i * (2048 >> 4)), idesc_o<T, kDim>(), !first || i > 0, lead);
+        attn_commit(&sh->pv_done[w], lead);
+        if (last) attn_commit(&sh->o_full[w], lead);
+    };
+    auto release = [&](uint32_t stage) { attn_commit(&sh->ring_empty[stage % kRing], lead); };
     auto queries = [&](int w) {
-        const bool ok = wait_bar(&sh->q_full[w], st.q[w] & 1u, sh, ctl, kErrAttnTile);
-        ++st.q[w];
+        const bool ok = __all_sync(0xffffffffu, wait_bar(&sh->q_full[w], st.q >> w & 1u, sh, ctl, kErrAttnTile));
+        st.q ^= 1u << w;
         return ok;
     };
-    auto weights = [&](int w) {
-        const bool ok = wait_bar(&sh->p_full[w], st.p[w] & 1u, sh, ctl, kErrAttnTile);
-        ++st.p[w];
+    auto weights = [&](int w, int b) {
+        const bool ok = __all_sync(0xffffffffu, wait_bar(&sh->p_full[w][b], st.p >> (2 * w + b) & 1u, sh, ctl, kErrAttnTile));
+        st.p ^= 1u << (2 * w + b);
         tc_fence_after();
         return ok;
     };
-    if (x.both) {
-        const int n = x.count[0];
-        if (n == 0) return;
-        for (int w = 0; w < 2; ++w)
-            if (!queries(w)) return;
-        if (!full(st.stage)) return;
-        tc_fence_after();
-        scores(0, st.stage);
-        scores(1, st.stage);
-        attn_commit(&sh->ring_empty[st.stage % kRing]);
-        ++st.stage;
-        for (int j = 0; j < n; ++j) {
-            const uint32_t v = st.stage++, k = st.stage;
-            const bool more = j + 1 < n;
-            if (more) ++st.stage;
-            for (int w = 0; w < 2; ++w) {
-                if (!weights(w)) return;
-                if (w == 0 && !full(v)) return;
-                tc_fence_after();
-                product(w, v, j > 0);
-                if (w == 1) attn_commit(&sh->ring_empty[v % kRing]);
-                if (more) {
-                    if (w == 0 && !full(k)) return;
-                    tc_fence_after();
-                    scores(w, k);
-                    if (w == 1) attn_commit(&sh->ring_empty[k % kRing]);
-                } else {
-                    attn_commit(&sh->o_full[w]);
+    uint32_t next = st.stage;                                  // the order of in_order()
+    if (both) {
+        const int n = n0;
+        if (n > 0 && (!queries(0) || !queries(1))) return false;
+#pragma unroll
+        for (int b = 0; b < 2; ++b) {
+            if (b >= n) break;
+            if (!full(next)) return false;
+            scores(0, b, next);
+            scores(1, b, next);
+            release(next++);
+        }
+        for (int s0 = 0; s0 < n; s0 += 2) {
+#pragma unroll
+            for (int b = 0; b < 2; ++b) {
+                const int s = s0 + b;
+                if (s >= n) break;
+                const bool more = s + 2 < n;
+                const uint32_t v = next++, k = next;
+                if (more) ++next;
+#pragma unroll
+                for (int w = 0; w < 2; ++w) {
+                    if (!weights(w, b) || (w == 0 && !full(v))) return false;
+                    product(w, b, v, s == 0, s + 1 == n);
+                    if (w == 1) release(v);
+                    if (!more) continue;
+                    if (w == 0 && !full(k)) return false;
+                    scores(w, b, k);
+                    if (w == 1) release(k);
                 }
             }
         }
-        return;
-    }
-    for (int w = 0; w < 2; ++w) {
-        if (x.count[w] == 0) continue;
-        if (!queries(w) || !full(st.stage)) return;
-        tc_fence_after();
-        scores(w, st.stage);
-        attn_commit(&sh->ring_empty[st.stage % kRing]);
-        ++st.stage;
-    }
-    for (int j = 0; j < max(x.count[0], x.count[1]); ++j)
+    } else {
+#pragma unroll
         for (int w = 0; w < 2; ++w) {
-            if (j >= x.count[w]) continue;
-            if (!weights(w) || !full(st.stage)) return;
-            tc_fence_after();
-            product(w, st.stage, j > 0);
-            attn_commit(&sh->ring_empty[st.stage % kRing]);
-            ++st.stage;
-            if (j + 1 < x.count[w]) {
-                if (!full(st.stage)) return;
-                tc_fence_after();
-                scores(w, st.stage);
-                attn_commit(&sh->ring_empty[st.stage % kRing]);
-                ++st.stage;
-            } else {
-                attn_commit(&sh->o_full[w]);
+            const int n = w == 0 ? n0 : n1;
+            if (n > 0 && !queries(w)) return false;
+#pragma unroll
+            for (int b = 0; b < 2; ++b) {
+                if (b >= n) break;
+                if (!full(next)) return false;
+                scores(w, b, next);
+                release(next++);
             }
         }
+        for (int s0 = 0; s0 < max(n0, n1); s0 += 2) {
+#pragma unroll
+            for (int b = 0; b < 2; ++b)
+#pragma unroll
+                for (int w = 0; w < 2; ++w) {
+                    const int s = s0 + b, n = w == 0 ? n0 : n1;
+                    if (s >= n) continue;
+                    if (!weights(w, b) || !full(next)) return false;
+                    product(w, b, next, s == 0, s + 1 == n);
+                    release(next++);
+                    if (s + 2 >= n) continue;
+                    if (!full(next)) return false;
+                    scores(w, b, next);
+                    release(next++);
+                }
+        }
+    }
+    st.stage = next;
+    return true;
 }
 
 // ---- workers (two groups of 128 threads) -------------------------------------------------------------------------
@@ -331,99 +378,112 @@ __device__ __forceinline__ void stage_queries(const AttnArgs &a, unsigned char *
     constexpr int kLanes = kDim / 8, kAtOnce = 32 / kLanes;
     const int lane = threadIdx.x & 31;
     const T *src = static_cast<const T *>(a.q) + (size_t)mine.token * a.q_stride + (size_t)(x.head * (int)a.group + mine.sub) * kDim;
-    const unsigned long long at = real ? (unsigned long long)src : 0ull;
-    const uint32_t flip = a.scale_log2 < 0.f ? 0x80008000u : 0u;
-#pragma unroll 4
-    for (int i = 0; i < 32; i += kAtOnce) {
-        const int r = i + lane / kLanes, chunk = lane % kLanes;
-        const unsigned long long p = __shfl_sync(0xffffffffu, at, r);
-        uint4 v = make_uint4(0, 0, 0, 0);
-        if (p != 0) v = __ldg(reinterpret_cast<const uint4 *>(p) + chunk);
-        v.x ^= flip; v.y ^= flip; v.z ^= flip; v.w ^= flip;
-        *reinterpret_cast<uint4 *>(dst + swz((uint32_t)(group_warp * 32 + r), (uint32_t)chunk, kTile)) = v;
+    const unsigned long long at = (unsigned long long)src;      // a row that is not real: some row's queries, thrown away
+    const uint32_t reals = __ballot_sync(0xffffffffu, real), flip = a.scale_log2 < 0.f ? 0x80008000u : 0u;
+    // All loads first, without conditions: one after another they would cost a round trip each.
+    uint4 v[32 / kAtOnce];
+#pragma unroll
+    for (int i = 0; i < 32 / kAtOnce; ++i)
+        v[i] = __ldg(reinterpret_cast<const uint4 *>(__shfl_sync(0xffffffffu, at, i * kAtOnce + lane / kLanes)) + lane % kLanes);
+#pragma unroll
+    for (int i = 0; i < 32 / kAtOnce; ++i) {
+        const int r = i * kAtOnce + lane / kLanes;
+        const bool keep = reals >> r & 1u;
+        v[i] = keep ? make_uint4(v[i].x ^ flip, v[i].y ^ flip, v[i].z ^ flip, v[i].w ^ flip) : make_uint4(0, 0, 0, 0);
+        *reinterpret_cast<uint4 *>(dst + swz((uint32_t)(group_warp * 32 + r), (uint32_t)(lane % kLanes), kTile)) = v[i];
     }
 }
 
+struct WorkState {
+    uint32_t stage;             // ring stages of the items so far
+    uint32_t s, o;              // parities to wait for: scores (bit: buffer), results
+    uint32_t pv, keys0, keys1;  // products of the group, and steps of both orders of keys, in the items so far
+    uint32_t bar;               // meetings of the group
+};
+
+// The four warps of a group meet; bounded like every wait, since a warp that gave up does not come.
+__device__ __forceinline__ bool group_meet(AttnShared *sh, Ctl *ctl, WorkState &st, int w) {
+    __syncwarp();
+    if ((threadIdx.x & 31) == 0) mbar_arrive(&sh->group_bar[w]);
+    return __all_sync(0xffffffffu, wait_bar(&sh->group_bar[w], st.bar++ & 1u, sh, ctl, kErrAttnTile));
+}
+
 template <class T, int kDim>
-__device__ __forceinline__ void work_tiles(const CacheView &c, const AttnArgs &a, AttnShared *sh, Ctl *ctl, unsigned char *smem_q, unsigned char *ring,
-                                           TileState &st, const TileItem &x) {
+__device__ __forceinline__ void work_tiles(const CacheView &c, const AttnArgs &a, const CUtensorMap *map_k, const CUtensorMap *map_v, AttnShared *sh,
+                                           Ctl *ctl, unsigned char *smem_q, unsigned char *ring, WorkState &st, Ring &units, const TileItem &x) {
     const int w = threadIdx.x >> 7, in_group = threadIdx.x & 127, warp = in_group >> 5, lane = threadIdx.x & 31;
+    if (!x.both && x.half == 1 && w == 1) {                   // no rows for the second group
+        st.stage += stages_of(x);
+        st.keys0 += x.steps0;
+        return;
+    }
     const int row = (x.both ? w * kTile : 0) + in_group;
     const bool real = row < x.rows;
     const RowOf mine = row_of(a, sh, x, real ? row : 0);
     const int limit = real ? min(mine.limit, x.end) : 0;
     const uint32_t tmem = *(volatile uint32_t *)&sh->tmem + ((uint32_t)(warp * 32) << 16);
-    const uint32_t ts = tmem + w * kTile, to = tmem + 2 * kTile + w * kDim;
+    const uint32_t to = tmem + 2 * kTile + w * kDim;
     const float scale = fmaxf(fabsf(a.scale_log2), 1e-30f);     // 0 would turn a hidden score into NaN
     float ref = -INFINITY, sum = 0.f;
-
-    // The smallest limit of the item's rows, and the stage of the ring that holds the group's next values.
+    // The smallest limit of the item's rows.
     int least = x.end;
     if (x.entry >= 0) least = min(least, sh->plan[x.entry].len - sh->plan[x.entry].t + x.r0 / (int)a.group + 1);
     const uint32_t stage0 = st.stage;
-    const int n = x.count[w];
+    const int n = w == 0 ? x.steps0 : x.steps1, pos0 = w == 0 ? x.pos0 : x.pos1, order = x.both ? 0 : w;
+    unsigned char *my_q = smem_q + w * query_bytes<kDim>();
     if (n > 0) {
-        stage_queries<T, kDim>(a, smem_q + w * tile_bytes<kDim>(), x, mine, real, warp);
+        stage_queries<T, kDim>(a, my_q, x, mine, real, warp);
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         __syncwarp();
         if (lane == 0) mbar_arrive(&sh->q_full[w]);
     }
-    bool ok = true;
-    for (int j = 0; j < n && ok; ++j) {
-        ok = __all_sync(0xffffffffu, wait_bar(&sh->s_full[w], st.s & 1u, sh, ctl, kErrAttnTile));
-        if (!ok) break;
-        ++st.s;
+    const int page_shift = min((int)c.page_shift, 6);            // of the part of a page that is in a step
+    const uint32_t whole = (1u << (kStep >> page_shift)) - 1u;
+    bool looked = false;                                        // some values were looked at: the group agrees on it
+    for (int s = 0; s < n; ++s) {
+        const uint32_t ts = tmem + w * kTile + (s & 1) * kStep;
+        const int pos = pos0 + s * kStep;
+        if (!__all_sync(0xffffffffu, wait_bar(&sh->s_full[w][s & 1], st.s >> (s & 1) & 1u, sh, ctl, kErrAttnTile))) return;
+        st.s ^= 1u << (s & 1);
         tc_fence_after();
-        uint32_t r[128];
+        uint32_t r[kStep];
+        tc_ld32(ts, *reinterpret_cast<uint32_t (*)[32]>(&r[0]));
+        tc_ld32(ts + 32, *reinterpret_cast<uint32_t (*)[32]>(&r[32]));
+        const uint32_t there = *(volatile uint32_t *)&sh->pages[order][((order == 0 ? st.keys0 : st.keys1) + s) % kPageWords];
+        tc_landed(r);
+        // Some row does not see some position: at the item's end, or where a page is not there.
+        if (pos + kStep > least || there != whole) {
+            const uint32_t vs = stage0 + v_stage(x, w, s);
+            if (!__all_sync(0xffffffffu, wait_bar(&sh->ring_full[vs % kRing], (vs / kRing) & 1u, sh, ctl, kErrAttnTile))) return;
+            unsigned char *v = ring + (size_t)(vs % kRing) * step_bytes<kDim>();
+            looked = true;
+            if (in_group < kStep) {                             // each thread looks after one position's values
+                const uint32_t at = (uint32_t)in_group;
+                if (pos + in_group >= x.end) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) tc_ld32(ts + i * 32, *reinterpret_cast<uint32_t (*)[32]>(&r[i * 32]));
-        tc_wait_ld();
-        // Where the group's V of this tile lies in the ring, in the order of loading.
-        const int pos = x.from + (x.first[w] + j) * kTile;
-        uint32_t vstage;
-        if (x.both) {
-            vstage = stage0 + 1 + 2 * j;
-        } else {
-            // stages before V_w(j): the first keys of both groups, then per tile and group a V and, but for the last, a K
-            vstage = stage0 + (x.count[0] > 0) + (x.count[1] > 0);
-            const int before0 = w == 0 ? j : j + 1, before1 = j;
-            vstage += min(before0, x.count[0]) + min(before0, max(x.count[0] - 1, 0));
-            vstage += min(before1, x.count[1]) + min(before1, max(x.count[1] - 1, 0));
-        }
-        // Some row does not see some position: the item's last tiles, or a page that is not there.  The pages of a tile are
-        // those of its V as well: the stage's word is read once V has arrived.
-        const bool edge = pos + kTile > least;
-        ok = __all_sync(0xffffffffu, wait_bar(&sh->ring_full[vstage % kRing], (vstage / kRing) & 1u, sh, ctl, kErrAttnTile));
-        if (!ok) break;
-        const uint32_t there = *(volatile uint32_t *)&sh->stage_pages[vstage % kRing];
-        const uint32_t whole = (1u << (kTile >> c.page_shift)) - 1u;
-        if (edge || there != whole) {
-            unsigned char *v = ring + (size_t)(vstage % kRing) * tile_bytes<kDim>();
-            const int at = pos + in_group;                    // each thread looks after one position's values
-            if (at >= x.end) {
-#pragma unroll
-                for (int i = 0; i < kDim / 8; ++i) *reinterpret_cast<uint4 *>(v + swz((uint32_t)in_group, (uint32_t)i, kTile)) = make_uint4(0, 0, 0, 0);
-                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-            } else if (at >= least) {
-                bool odd = false;
+                    for (int i = 0; i < kDim / 8; ++i) *reinterpret_cast<uint4 *>(v + swz(at, (uint32_t)i, kStep)) = make_uint4(0, 0, 0, 0);
+                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                } else if (pos + in_group >= least) {
+                    bool odd = false;
 #pragma unroll 4
-                for (int i = 0; i < kDim / 8; ++i) {
-                    const uint4 y = *reinterpret_cast<const uint4 *>(v + swz((uint32_t)in_group, (uint32_t)i, kTile));
-                    const uint32_t z[4] = {y.x, y.y, y.z, y.w};
+                    for (int i = 0; i < kDim / 8; ++i) {
+                        const uint4 y = *reinterpret_cast<const uint4 *>(v + swz(at, (uint32_t)i, kStep));
+                        const uint32_t z[4] = {y.x, y.y, y.z, y.w};
 #pragma unroll
-                    for (int k = 0; k < 4; ++k)
-                        odd |= (z[k] & Elem<T>::kInfBits) == Elem<T>::kInfBits || (z[k] >> 16 & Elem<T>::kInfBits) == Elem<T>::kInfBits;
+                        for (int k = 0; k < 4; ++k)
+                            odd |= (z[k] & Elem<T>::kInfBits) == Elem<T>::kInfBits || (z[k] >> 16 & Elem<T>::kInfBits) == Elem<T>::kInfBits;
+                    }
+                    if (odd) *(volatile uint32_t *)&sh->odd[w] = 1u;
                 }
-                if (odd) *(volatile uint32_t *)&sh->odd = 1u;
             }
             const int seen = limit - pos;
 #pragma unroll
-            for (int i = 0; i < 128; ++i)
-                if (i >= seen || !(there >> (i >> c.page_shift) & 1u)) r[i] = 0xff800000u;
+            for (int i = 0; i < kStep; ++i)
+                if (i >= seen || !(there >> (i >> page_shift) & 1u)) r[i] = 0xff800000u;
         }
         float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-        for (int i = 0; i < 128; i += 4)
+        for (int i = 0; i < kStep; i += 4)
 #pragma unroll
             for (int k = 0; k < 4; ++k) top[k] = fmaxf(top[k], __uint_as_float(r[i + k]));
         const float most = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
@@ -433,106 +493,133 @@ __device__ __forceinline__ void work_tiles(const CacheView &c, const AttnArgs &a
             ref = most;
         }
         const float base = ref == -INFINITY ? 0.f : ref * scale;
-        if (j > 0 && __any_sync(0xffffffffu, down != 1.f)) {
+        if (s > 0 && __any_sync(0xffffffffu, down != 1.f)) {    // O stands still once the product before this step is done (the one before that is)
+            if (!__all_sync(0xffffffffu, wait_bar(&sh->pv_done[w], (st.pv + s - 1) & 1u, sh, ctl, kErrAttnTile))) return;
+            tc_fence_after();
             sum *= down;
 #pragma unroll 1
             for (int i = 0; i < kDim; i += 32) {
                 uint32_t o[32];
                 tc_ld32(to + i, o);
-                tc_wait_ld();
+                tc_landed(o);
 #pragma unroll
                 for (int k = 0; k < 32; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * down);
                 tc_st32(to + i, o);
             }
         }
         float part[4] = {0.f, 0.f, 0.f, 0.f};
+        uint32_t p[32];
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            uint32_t p[32];
-#pragma unroll
-            for (int i = 0; i < 32; ++i) {
-                const float e0 = ex2(fmaf(__uint_as_float(r[h * 64 + 2 * i]), scale, -base));
-                const float e1 = ex2(fmaf(__uint_as_float(r[h * 64 + 2 * i + 1]), scale, -base));
-                part[(2 * i) & 3] += e0;
-                part[(2 * i + 1) & 3] += e1;
-                p[i] = Elem<T>::pack(e0, e1);
-            }
-            tc_st32(ts + h * 32, p);
+        for (int i = 0; i < 32; ++i) {
+            const float e0 = ex2(fmaf(__uint_as_float(r[2 * i]), scale, -base)), e1 = ex2(fmaf(__uint_as_float(r[2 * i + 1]), scale, -base));
+            part[(2 * i) & 3] += e0;
+            part[(2 * i + 1) & 3] += e1;
+            p[i] = Elem<T>::pack(e0, e1);
         }
+        tc_st32(ts, p);
         tc_wait_st();
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&sh->p_full[w]);
+        if (lane == 0) mbar_arrive(&sh->p_full[w][s & 1]);
         sum += (part[0] + part[1]) + (part[2] + part[3]);
     }
-    // All stages of the item have been asked for, whether or not this group used them.
-    const int k0 = x.count[0], k1 = x.both ? 0 : x.count[1];
-    st.stage = stage0 + 2 * (k0 + k1);
-    if (!ok) return;
-
-    const float inv = sum == 0.f ? 0.f : 1.f / sum;
+    st.stage = stage0 + stages_of(x);
+    st.keys0 += x.steps0;
+    if (!x.both) st.keys1 += x.steps1;
     if (n > 0) {
-        ok = __all_sync(0xffffffffu, wait_bar(&sh->o_full[w], st.o & 1u, sh, ctl, kErrAttnTile));
-        if (!ok) return;
-        ++st.o;
+        if (!__all_sync(0xffffffffu, wait_bar(&sh->o_full[w], st.o, sh, ctl, kErrAttnTile))) return;
+        st.o ^= 1u;
+        st.pv += n;
         tc_fence_after();
     }
     const bool direct = x.slot0 < 0;
-    // Row r of the item belongs to group r / 16, the second workers' half to the slot behind.  Without tiles the result is empty.
-    if (w == 1 && !x.both && x.half == 1) return;            // no rows for the second group
-    const size_t slot = direct ? 0 : (size_t)(x.slot0 + row / kUnitRows * x.step + (x.half == 2 ? w : 0));
-    const size_t place = slot * kUnitRows + row % kUnitRows;
-    if (!direct && real) __stcg(a.part_ml + place, n > 0 ? make_float2(ref == -INFINITY ? -INFINITY : ref * scale, sum) : make_float2(-INFINITY, 0.f));
-    T *out = static_cast<T *>(a.out) + (size_t)mine.token * a.out_stride + (size_t)(x.head * (int)a.group + mine.sub) * kDim;
-    float *part = a.part + place * kDim;
-#pragma unroll 1
-    for (int i = 0; i < kDim; i += 32) {
-        uint32_t o[32];
-        if (n > 0) {
-            tc_ld32(to + i, o);
-            tc_wait_ld();
-        } else {
-            if (!direct) break;
+    bool again = false;
+    if (looked) {                                               // were the values that somebody did not see all finite?
+        if (!group_meet(sh, ctl, st, w)) return;
+        again = *(volatile uint32_t *)&sh->odd[w] != 0u;
+        if (!group_meet(sh, ctl, st, w)) return;
+        if (in_group == 0) sh->odd[w] = 0;                      // nobody looks again before this warp's next queries are there
+    }
+    if (!again) {
+        // Row r of the item belongs to group r / 16, the second workers' half to the slot behind.  Without steps the result is empty.
+        const float inv = sum == 0.f ? 0.f : 1.f / sum;
+        const size_t slot = direct ? 0 : (size_t)(x.slot0 + row / kUnitRows * x.step + (x.half == 2 ? w : 0));
+        const size_t place = slot * kUnitRows + row % kUnitRows;
+        if (!direct && real) __stcg(a.part_ml + place, n > 0 ? make_float2(ref == -INFINITY ? -INFINITY : ref * scale, sum) : make_float2(-INFINITY, 0.f));
+        // A thread has a row, a store instruction wants consecutive bytes: rows pass through the group's queries (nobody reads them any
+        // more), each warp through its own 32.
+        const unsigned long long to_row = direct ? (unsigned long long)(static_cast<T *>(a.out) + (size_t)mine.token * a.out_stride
+                                                                        + (size_t)(x.head * (int)a.group + mine.sub) * kDim)
+                                                 : (unsigned long long)(a.part + place * kDim);
+        const uint32_t reals = __ballot_sync(0xffffffffu, real);
+        auto out_rows = [&](auto width, int skip) {             // `width` 16-byte chunks of each row, from byte `skip` of it
+            constexpr int kChunks = decltype(width)::value, kRows = 32 / kChunks;
+            __syncwarp();
 #pragma unroll
-            for (int k = 0; k < 32; ++k) o[k] = 0;
-        }
-        if (!real) continue;
-        if (direct) {
-#pragma unroll
-            for (int k = 0; k < 32; k += 8) {
-                uint32_t y[4];
-#pragma unroll
-                for (int m = 0; m < 4; ++m)
-                    y[m] = sum == 0.f ? 0u : Elem<T>::pack(__uint_as_float(o[k + 2 * m]) * inv, __uint_as_float(o[k + 2 * m + 1]) * inv);
-                *reinterpret_cast<uint4 *>(out + i + k) = make_uint4(y[0], y[1], y[2], y[3]);
+            for (int i = 0; i < kChunks; ++i) {
+                const int r = i * kRows + lane / kChunks;
+                const uint4 y = *reinterpret_cast<const uint4 *>(my_q + swz((uint32_t)(warp * 32 + r), (uint32_t)(lane % kChunks), kTile));
+                const unsigned long long p = __shfl_sync(0xffffffffu, to_row, r);
+                if (reals >> r & 1u) __stcg(reinterpret_cast<uint4 *>(p + skip) + lane % kChunks, y);
             }
-        } else {
+            __syncwarp();
+        };
+        if (direct) {
+#pragma unroll 1
+            for (int i = 0; i < kDim; i += 32) {
+                uint32_t o[32];
+                if (n > 0) tc_ld32(to + i, o);
+                tc_landed(o);
 #pragma unroll
-            for (int k = 0; k < 32; k += 4)
-                __stcg(reinterpret_cast<float4 *>(part + i + k), make_float4(__uint_as_float(o[k]), __uint_as_float(o[k + 1]), __uint_as_float(o[k + 2]),
-                                                                           __uint_as_float(o[k + 3])));
+                for (int k = 0; k < 32; k += 8) {
+                    uint32_t y[4];
+#pragma unroll
+                    for (int m = 0; m < 4; ++m)
+                        y[m] = sum == 0.f ? 0u : Elem<T>::pack(__uint_as_float(o[k + 2 * m]) * inv, __uint_as_float(o[k + 2 * m + 1]) * inv);
+                    *reinterpret_cast<uint4 *>(my_q + swz((uint32_t)in_group, (uint32_t)((i + k) / 8), kTile)) = make_uint4(y[0], y[1], y[2], y[3]);
+                }
+            }
+            out_rows(std::integral_constant<int, kDim / 8>(), 0);
+        } else if (n > 0) {
+            constexpr int kPass = query_bytes<kDim>() / kTile / 4;          // elements of a row that fit at a time
+#pragma unroll 1
+            for (int at = 0; at < kDim; at += kPass) {
+#pragma unroll 1
+                for (int i = 0; i < kPass; i += 32) {
+                    uint32_t o[32];
+                    tc_ld32(to + at + i, o);
+                    tc_landed(o);
+#pragma unroll
+                    for (int k = 0; k < 32; k += 4)
+                        *reinterpret_cast<uint4 *>(my_q + swz((uint32_t)in_group, (uint32_t)((i + k) / 4), kTile)) = make_uint4(o[k], o[k + 1], o[k + 2], o[k + 3]);
+                }
+                out_rows(std::integral_constant<int, kPass / 4>(), at * 4);
+            }
         }
+    } else {
+        // Hidden values that are not finite: the group's rows once more by units, which add such values with selects.  Their rings lie
+        // where the group's queries were (a stage each), which nobody reads any more.
+        units.move(my_q + warp * unit_stage_bytes<kDim>(), 1);
+        for (int i = (x.both ? w * (kTile / kUnitRows) : 0) + warp; i < x.groups && i < (x.both ? (w + 1) * (kTile / kUnitRows) : x.groups); i += 4) {
+            Unit u;
+            u.entry = x.entry;
+            u.head = x.head;
+            u.r0 = x.r0 + i * kUnitRows;
+            u.rows = min(kUnitRows, x.rows - i * kUnitRows);
+            u.from = x.from;
+            u.first = (pos0 - x.from) / kBlock;
+            u.last = min(u.first + n * (kStep / kBlock), (x.end - x.from + kBlock - 1) / kBlock);
+            u.slot = direct ? -1 : x.slot0 + i * x.step + (x.half == 2 ? w : 0);
+            run_unit<T, kDim, 2>(c, a, map_k, map_v, sh, ctl, units, u);
+        }
+        if (!group_meet(sh, ctl, st, w)) return;                // the next queries may come
     }
     tc_fence_before();
-}
-
-// An item whose hidden values were not finite, once more by units (which add such values with selects).
-template <class T, int kDim>
-__device__ __forceinline__ void redo_item(const CacheView &c, const AttnArgs &a, const CUtensorMap *map_k, const CUtensorMap *map_v, AttnShared *sh,
-                                          Ctl *ctl, Ring &r, const TileItem &x) {
-    const int parts = x.half;
-    for (int i = threadIdx.x >> 5; i < x.groups * parts; i += kWorkers) {
-        const int g = i / parts, h = i % parts;
-        Unit u;
-        u.entry = x.entry;
-        u.head = x.head;
-        u.r0 = x.r0 + g * kUnitRows;
-        u.rows = min(kUnitRows, x.rows - g * kUnitRows);
-        u.from = x.from;
-        u.first = x.first[h] * (kTile / kBlock);
-        u.last = min((x.first[h] + x.count[h]) * (kTile / kBlock), (x.end - x.from + kBlock - 1) / kBlock);
-        u.slot = x.slot0 < 0 ? -1 : x.slot0 + g * x.step + h;
-        run_unit<T, kDim, 2>(c, a, map_k, map_v, sh, ctl, r, u);
+    if (!direct) {                                              // tell the merges how many row groups have their result
+        __threadfence();
+        if (!group_meet(sh, ctl, st, w)) return;
+        const int mine_groups = x.half == 2 ? x.groups : max(min(x.groups - w * (kTile / kUnitRows), kTile / kUnitRows), 0);
+        if (in_group == 64) atomicAdd(&a.counters[(size_t)(x.entry < 0 ? (int)a.n : x.entry) * c.heads + x.head], (uint32_t)mine_groups);
     }
 }
 

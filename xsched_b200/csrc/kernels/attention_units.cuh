@@ -9,10 +9,29 @@
 
 namespace xpk {
 
-struct Ring {                 // one warp's ring of blocks
+// One warp's ring of blocks.  Its place and depth change with what the CTA is doing; a stage's phase goes with its barrier.
+struct Ring {
     unsigned char *smem;
     unsigned long long *full;
-    uint32_t loaded, used;    // blocks asked for and consumed since the kernel began
+    uint32_t stages;
+    uint32_t loading, using_;      // next stage to fill and to read
+    uint32_t phases, pending;      // bit s: parity to wait for at stage s; loads not yet waited for
+
+    __device__ __forceinline__ void move(unsigned char *to, uint32_t depth) { smem = to; stages = depth; loading = using_ = 0; }
+    __device__ __forceinline__ uint32_t take() {
+        const uint32_t s = loading;
+        loading = s + 1 == stages ? 0 : s + 1;
+        ++pending;
+        return s;
+    }
+    __device__ __forceinline__ uint32_t parity() const { return phases >> using_ & 1u; }
+    __device__ __forceinline__ uint32_t give() {
+        const uint32_t s = using_;
+        phases ^= 1u << s;
+        using_ = s + 1 == stages ? 0 : s + 1;
+        --pending;
+        return s;
+    }
 };
 
 // What a unit covers: 16 rows of an entry for one key head, blocks [first, last) counted from its position `from`.
@@ -84,8 +103,8 @@ __device__ __forceinline__ void run_unit(const CacheView &c, const AttnArgs &a, 
             const int id = __shfl_sync(0xffffffffu, load_ids, next_load - load_base);
             const int b = next_load++;
             if (id < 0) continue;
+            const uint32_t s = ring.take();
             if (lane == 0) {
-                const uint32_t s = ring.loaded % kUnitStages;
                 unsigned char *dst = ring.smem + s * kStage;
                 mbar_arrive_expect_tx(&ring.full[s], kStage);
                 const int y = head * (int)c.page + ((w.from + b * kBlock) & (int)(c.page - 1)), z = (int)(a.layer * c.pages) + id;
@@ -95,20 +114,18 @@ __device__ __forceinline__ void run_unit(const CacheView &c, const AttnArgs &a, 
                     tma_load_3d(dst + kHalf + x * 2 * kBlock, map_v, &ring.full[s], x, y, z);
                 }
             }
-            ++ring.loaded;
             return;
         }
     };
-    for (int s = 0; s < kUnitStages; ++s) issue();
+    for (uint32_t s = 0; s < ring.stages; ++s) issue();
 
     bool ok = true;
     for (int b = first_block; b < last_block; ++b) {
         if (b - use_base >= 32) { use_base += 32; use_ids = page_ids(use_base); }
         if (__shfl_sync(0xffffffffu, use_ids, b - use_base) < 0) continue;
-        const uint32_t s = ring.used % kUnitStages, phase = (ring.used / kUnitStages) & 1u;
-        ok = __all_sync(0xffffffffu, wait_bar(&ring.full[s], phase, sh, ctl, kErrAttnLoad));
+        ok = __all_sync(0xffffffffu, wait_bar(&ring.full[ring.using_], ring.parity(), sh, ctl, kErrAttnLoad));
         if (!ok) break;
-        ++ring.used;
+        const uint32_t s = ring.give();
         unsigned char *stage = ring.smem + s * kStage;
         const uint32_t ka = smem_u32(stage), va = ka + kHalf;
         const int pos0 = w.from + b * kBlock;
@@ -259,12 +276,12 @@ __device__ __forceinline__ void unit_ticket(const CacheView &c, const AttnArgs &
         if (sh->unit0[mid] <= ticket) lo = mid; else hi = mid - 1;
     }
     const SeqPlan p = sh->plan[lo];
-    const int runs = runs_of(sh, a.group, lo), local = ticket - sh->unit0[lo], run = local % runs;
+    const int runs = runs_of(sh, a.group, lo), groups = row_groups(rows_of(p, a.group)), local = ticket - sh->unit0[lo], run = local % runs;
     Unit w;
     w.entry = lo;
-    w.head = local / runs;
-    w.r0 = 0;
-    w.rows = (int)rows_of(p, a.group);
+    w.head = local / (runs * groups);
+    w.r0 = local / runs % groups * kUnitRows;
+    w.rows = (int)min(rows_of(p, a.group) - w.r0, (long long)kUnitRows);
     w.from = own_from(sh, lo);
     w.first = run * sh->run;
     w.last = min(w.first + sh->run, (p.len - w.from + kBlock - 1) / kBlock);
@@ -346,19 +363,28 @@ __device__ __forceinline__ void run_merge(const CacheView &c, const AttnArgs &a,
             const float w = ml.x == -INFINITY && ml.y == 0.f ? -1.f : ex2(ml.x - base);
             if (!(w < 0.f)) sum = fmaf(w, ml.y, sum);
             const int here = min(32, all - b);
-#pragma unroll 4
-            for (int i = 0; i < here; ++i) {
-                const float wi = __shfl_sync(0xffffffffu, w, i);
-                if (wi < 0.f) continue;
-                const float *src = a.part + at(b + i) * kDim + lane * kVec;
-                if constexpr (kVec == 4) {
-                    const float4 x = __ldcg(reinterpret_cast<const float4 *>(src));
-                    acc[0] = fmaf(wi, x.x, acc[0]); acc[1] = fmaf(wi, x.y, acc[1]);
-                    acc[2] = fmaf(wi, x.z, acc[2]); acc[3] = fmaf(wi, x.w, acc[3]);
-                } else {
-                    const float2 x = __ldcg(reinterpret_cast<const float2 *>(src));
-                    acc[0] = fmaf(wi, x.x, acc[0]); acc[1] = fmaf(wi, x.y, acc[1]);
+            // Eight results in flight: one after another they would cost an L2 round trip each.
+            for (int i0 = 0; i0 < here; i0 += 8) {
+                float x[8][kVec], wi[8];
+#pragma unroll
+                for (int u = 0; u < 8; ++u) {
+                    const int i = min(i0 + u, 31);
+                    wi[u] = __shfl_sync(0xffffffffu, w, i);
+                    const bool real = i0 + u < here && !(wi[u] < 0.f);
+                    if (!real) wi[u] = 0.f;
+                    const float *src = a.part + at(real ? b + i : 0) * kDim + lane * kVec;
+                    if constexpr (kVec == 4) {
+                        const float4 y = real ? __ldcg(reinterpret_cast<const float4 *>(src)) : make_float4(0.f, 0.f, 0.f, 0.f);
+                        x[u][0] = y.x; x[u][1] = y.y; x[u][2] = y.z; x[u][3] = y.w;
+                    } else {
+                        const float2 y = real ? __ldcg(reinterpret_cast<const float2 *>(src)) : make_float2(0.f, 0.f);
+                        x[u][0] = y.x; x[u][1] = y.y;
+                    }
                 }
+#pragma unroll
+                for (int u = 0; u < 8; ++u)
+#pragma unroll
+                    for (int v = 0; v < kVec; ++v) acc[v] = fmaf(wi[u], x[u][v], acc[v]);
             }
         }
 #pragma unroll

@@ -3,6 +3,7 @@
 #include "kv_cache.cuh"
 
 #include <cuda.h>
+#include <algorithm>
 #include <cmath>
 #include <cstring>
 #include <mutex>
@@ -121,7 +122,7 @@ xpkResult xpkKvCacheCreate(xpkKvCache_t *cache, const xpkKvCacheDesc *desc) {
     const size_t bytes = xpk::kv_work_bytes(d.pages);
     if (cudaMalloc((void **)&c->work, bytes) != cudaSuccess || cudaMemset(c->work, 0, bytes) != cudaSuccess) { free_cache(c); return XPK_ERR_CUDA; }
     if (!pool_map(c->map_k, d, d.k, 16) || !pool_map(c->map_v, d, d.v, 16) ||
-        !pool_map(c->page_k, d, d.k, d.page_size) || !pool_map(c->page_v, d, d.v, d.page_size)) { free_cache(c); return XPK_ERR_CUDA; }
+        !pool_map(c->page_k, d, d.k, std::min(d.page_size, 64u)) || !pool_map(c->page_v, d, d.v, std::min(d.page_size, 64u))) { free_cache(c); return XPK_ERR_CUDA; }
     const xpkResult r = attention_ready(c->device);
     if (r != XPK_SUCCESS) { free_cache(c); return r; }
     *cache = c;

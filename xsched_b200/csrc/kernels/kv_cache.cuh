@@ -8,7 +8,7 @@ struct xpkKvCache_st {
     int sms = 0;
     int32_t *work = nullptr;              // see KvWork
     alignas(64) unsigned char map_k[128], map_v[128];      // boxes of 16 positions x 64 elements
-    alignas(64) unsigned char page_k[128], page_v[128];    // boxes of a page x 64 elements
+    alignas(64) unsigned char page_k[128], page_v[128];    // boxes of a page (64 positions at most) x 64 elements
 };
 
 namespace xpk {
