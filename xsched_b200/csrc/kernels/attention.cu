@@ -197,8 +197,8 @@ __device__ __forceinline__ void work_off(Ctl *ctl, const CUtensorMap *map_k, con
 template <class T, int kDim, bool kPreemptible>
 __global__ void __launch_bounds__(kAttnThreads, 1)
 attention_kernel(Ctl *ctl, const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
-                 const __grid_constant__ CUtensorMap page_k, const __grid_constant__ CUtensorMap page_v, CacheView c, AttnArgs a,
-                 unsigned long long launch_no) {
+                 const __grid_constant__ CUtensorMap page_k, const __grid_constant__ CUtensorMap page_v,
+                 const __grid_constant__ CacheView c, const __grid_constant__ AttnArgs a, unsigned long long launch_no) {
     extern __shared__ unsigned char smem_raw[];
     unsigned char *smem = (unsigned char *)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
     AttnShared *sh = reinterpret_cast<AttnShared *>(smem + ring_bytes<kDim>());

@@ -16,7 +16,7 @@ constexpr int kBlock = 16;                                  // positions per blo
 constexpr int kUnitRows = 16;                               // rows of a unit, and of a partial result
 constexpr int kUnitRowsMost = 32;                           // sequences of more rows go by tiles
 constexpr int kUnitStages = 3;
-constexpr int kUnitWaves = 4;                               // units that each warp gets where there is enough work
+constexpr int kUnitWaves = 2;                               // units that each warp gets where there is enough work
 constexpr int kTile = 128;                                  // positions per tile; rows per group of a tile item
 constexpr int kItemRows = 2 * kTile;
 constexpr int kStep = 64;                                   // positions per product; tiles are counted in pairs of steps

@@ -47,6 +47,17 @@ __device__ __forceinline__ void attn_mma_ts(uint32_t d, uint32_t a, uint64_t b, 
                  "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
                  :: "r"(d), "r"(a), "l"(b), "r"(idesc), "r"(accumulate), "r"(lead) : "memory");
 }
+__device__ __forceinline__ void tc_ld16(uint32_t taddr, uint32_t (&r)[16]) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+                   "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+                 : "r"(taddr) : "memory");
+}
+__device__ __forceinline__ void tc_st16(uint32_t taddr, const uint32_t (&r)[16]) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15};"
+                 :: "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]),
+                    "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(taddr) : "memory");
+}
 __device__ __forceinline__ void tc_st32(uint32_t taddr, const uint32_t *r) {
     asm volatile("tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], "
                  "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
@@ -59,13 +70,44 @@ __device__ __forceinline__ void tc_st32(uint32_t taddr, const uint32_t *r) {
 // Waits for loads from tensor memory.  The registers pass through an empty statement behind the wait: arithmetic on them has
 // no other reason to stay behind it.
 template <int N>
-__device__ __forceinline__ void tc_landed(uint32_t (&r)[N]) {
-    tc_wait_ld();
+__device__ __forceinline__ void tc_pin(uint32_t (&r)[N]) {
 #pragma unroll
     for (int i = 0; i < N; i += 8)
         asm volatile("" : "+r"(r[i]), "+r"(r[i + 1]), "+r"(r[i + 2]), "+r"(r[i + 3]), "+r"(r[i + 4]), "+r"(r[i + 5]), "+r"(r[i + 6]), "+r"(r[i + 7]));
 }
+template <int N>
+__device__ __forceinline__ void tc_landed(uint32_t (&r)[N]) {
+    tc_wait_ld();
+    tc_pin(r);
+}
 __device__ __forceinline__ void tc_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+// Two fp32 operations an instruction.
+__device__ __forceinline__ uint64_t two(float a, float b) {
+    uint64_t x;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(x) : "f"(a), "f"(b));
+    return x;
+}
+__device__ __forceinline__ float2 of_two(uint64_t x) {
+    float2 y;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(y.x), "=f"(y.y) : "l"(x));
+    return y;
+}
+__device__ __forceinline__ uint64_t fma_two(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t d;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+    return d;
+}
+__device__ __forceinline__ uint64_t mul_two(uint64_t a, uint64_t b) {
+    uint64_t d;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+    return d;
+}
+__device__ __forceinline__ uint64_t add_two(uint64_t a, uint64_t b) {
+    uint64_t d;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+    return d;
+}
 
 // V as B operand with the dimension contiguous: atoms of 64 dimensions x 8 positions (1024 B, 128-byte swizzle), the next
 // eight positions behind it, the next 64 dimensions a whole step of 64 positions further.
@@ -282,14 +324,20 @@ __device__ __forceinline__ bool issue_steps(AttnShared *sh, Ctl *ctl, unsigned c
     uint32_t next = st.stage;                                  // the order of in_order()
     if (both) {
         const int n = n0;
-        if (n > 0 && (!queries(0) || !queries(1))) return false;
+        if (n > 0 && !queries(0)) return false;
+        const uint32_t first = next;
 #pragma unroll
         for (int b = 0; b < 2; ++b) {
             if (b >= n) break;
             if (!full(next)) return false;
-            scores(0, b, next);
-            scores(1, b, next);
-            release(next++);
+            scores(0, b, next++);
+        }
+        if (n > 0 && !queries(1)) return false;
+#pragma unroll
+        for (int b = 0; b < 2; ++b) {
+            if (b >= n) break;
+            scores(1, b, first + b);
+            release(first + b);
         }
         for (int s0 = 0; s0 < n; s0 += 2) {
 #pragma unroll
@@ -408,6 +456,27 @@ __device__ __forceinline__ bool group_meet(AttnShared *sh, Ctl *ctl, WorkState &
     return __all_sync(0xffffffffu, wait_bar(&sh->group_bar[w], st.bar++ & 1u, sh, ctl, kErrAttnTile));
 }
 
+// A group's rows of an item by units, which add values that are not finite with selects.  Their rings lie where the group's queries
+// were (a stage each), which nobody reads any more.  Not inlined: it never runs on sane data and would cost the loop registers.
+template <class T, int kDim>
+__device__ __noinline__ void redo_rows(const CacheView &c, const AttnArgs &a, const CUtensorMap *map_k, const CUtensorMap *map_v, AttnShared *sh, Ctl *ctl,
+                                       unsigned char *place, Ring &units, const TileItem &x, int w, int warp, int pos0, int steps) {
+    units.move(place + warp * unit_stage_bytes<kDim>(), 1);
+    const int begin = x.both ? w * (kTile / kUnitRows) : 0, end = x.both ? min(x.groups, begin + kTile / kUnitRows) : x.groups;
+    for (int i = begin + warp; i < end; i += 4) {
+        Unit u;
+        u.entry = x.entry;
+        u.head = x.head;
+        u.r0 = x.r0 + i * kUnitRows;
+        u.rows = min(kUnitRows, x.rows - i * kUnitRows);
+        u.from = x.from;
+        u.first = (pos0 - x.from) / kBlock;
+        u.last = min(u.first + steps * (kStep / kBlock), (x.end - x.from + kBlock - 1) / kBlock);
+        u.slot = x.slot0 < 0 ? -1 : x.slot0 + i * x.step + (x.half == 2 ? w : 0);
+        run_unit<T, kDim, 2>(c, a, map_k, map_v, sh, ctl, units, u);
+    }
+}
+
 template <class T, int kDim>
 __device__ __forceinline__ void work_tiles(const CacheView &c, const AttnArgs &a, const CUtensorMap *map_k, const CUtensorMap *map_v, AttnShared *sh,
                                            Ctl *ctl, unsigned char *smem_q, unsigned char *ring, WorkState &st, Ring &units, const TileItem &x) {
@@ -424,7 +493,7 @@ __device__ __forceinline__ void work_tiles(const CacheView &c, const AttnArgs &a
     const uint32_t tmem = *(volatile uint32_t *)&sh->tmem + ((uint32_t)(warp * 32) << 16);
     const uint32_t to = tmem + 2 * kTile + w * kDim;
     const float scale = fmaxf(fabsf(a.scale_log2), 1e-30f);     // 0 would turn a hidden score into NaN
-    float ref = -INFINITY, sum = 0.f;
+    float ref = -INFINITY;
     // The smallest limit of the item's rows.
     int least = x.end;
     if (x.entry >= 0) least = min(least, sh->plan[x.entry].len - sh->plan[x.entry].t + x.r0 / (int)a.group + 1);
@@ -440,17 +509,39 @@ __device__ __forceinline__ void work_tiles(const CacheView &c, const AttnArgs &a
     const int page_shift = min((int)c.page_shift, 6);            // of the part of a page that is in a step
     const uint32_t whole = (1u << (kStep >> page_shift)) - 1u;
     bool looked = false;                                        // some values were looked at: the group agrees on it
-    for (int s = 0; s < n; ++s) {
-        const uint32_t ts = tmem + w * kTile + (s & 1) * kStep;
-        const int pos = pos0 + s * kStep;
-        if (!__all_sync(0xffffffffu, wait_bar(&sh->s_full[w][s & 1], st.s >> (s & 1) & 1u, sh, ctl, kErrAttnTile))) return;
+    // A step: maximum, then exponentials of the first 32 scores; their registers are free for the next step's, whose load runs under the
+    // other 32 and under the store of the weights.
+    uint32_t lo[32], hi[32], p[32];
+    uint64_t part = 0ull;
+    float base = 0.f;                                           // ref * scale, 0 while nothing was seen
+    const uint64_t scale2 = two(scale, scale);
+    auto scores = [&](int s) { return tmem + w * kTile + (s & 1) * kStep; };
+    auto ready = [&](int s) {
+        const bool ok = __all_sync(0xffffffffu, wait_bar(&sh->s_full[w][s & 1], st.s >> (s & 1) & 1u, sh, ctl, kErrAttnTile));
         st.s ^= 1u << (s & 1);
         tc_fence_after();
-        uint32_t r[kStep];
-        tc_ld32(ts, *reinterpret_cast<uint32_t (*)[32]>(&r[0]));
-        tc_ld32(ts + 32, *reinterpret_cast<uint32_t (*)[32]>(&r[32]));
+        return ok;
+    };
+    auto exps = [&](const uint32_t (&r)[32], int at) {
+        const uint64_t base2 = two(-base, -base);
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            const float2 e = of_two(fma_two(two(__uint_as_float(r[2 * i]), __uint_as_float(r[2 * i + 1])), scale2, base2));
+            const float e0 = ex2(e.x), e1 = ex2(e.y);
+            part = add_two(part, two(e0, e1));
+            p[at + i] = Elem<T>::pack(e0, e1);
+        }
+    };
+    if (n > 0) {
+        if (!ready(0)) return;
+        tc_ld32(scores(0), lo);
+        tc_ld32(scores(0) + 32, hi);
+        tc_landed(lo);
+        tc_pin(hi);
+    }
+    for (int s = 0; s < n; ++s) {
+        const int pos = pos0 + s * kStep;
         const uint32_t there = *(volatile uint32_t *)&sh->pages[order][((order == 0 ? st.keys0 : st.keys1) + s) % kPageWords];
-        tc_landed(r);
         // Some row does not see some position: at the item's end, or where a page is not there.
         if (pos + kStep > least || there != whole) {
             const uint32_t vs = stage0 + v_stage(x, w, s);
@@ -479,50 +570,54 @@ __device__ __forceinline__ void work_tiles(const CacheView &c, const AttnArgs &a
             const int seen = limit - pos;
 #pragma unroll
             for (int i = 0; i < kStep; ++i)
-                if (i >= seen || !(there >> (i >> page_shift) & 1u)) r[i] = 0xff800000u;
+                if (i >= seen || !(there >> (i >> page_shift) & 1u)) (i < 32 ? lo[i & 31] : hi[i & 31]) = 0xff800000u;
         }
         float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-        for (int i = 0; i < kStep; i += 4)
+        for (int i = 0; i < 32; i += 4)
 #pragma unroll
-            for (int k = 0; k < 4; ++k) top[k] = fmaxf(top[k], __uint_as_float(r[i + k]));
+            for (int k = 0; k < 4; ++k) top[k] = fmaxf(fmaxf(top[k], __uint_as_float(lo[i + k])), __uint_as_float(hi[i + k]));
         const float most = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
-        float down = 1.f;
-        if (most > ref && (ref == -INFINITY || (most - ref) * scale > kLag)) {
-            down = ref == -INFINITY ? 0.f : ex2((ref - most) * scale);
-            ref = most;
-        }
-        const float base = ref == -INFINITY ? 0.f : ref * scale;
-        if (s > 0 && __any_sync(0xffffffffu, down != 1.f)) {    // O stands still once the product before this step is done (the one before that is)
-            if (!__all_sync(0xffffffffu, wait_bar(&sh->pv_done[w], (st.pv + s - 1) & 1u, sh, ctl, kErrAttnTile))) return;
-            tc_fence_after();
-            sum *= down;
+        // (-inf) - (-inf) is no reason to move.
+        if (__any_sync(0xffffffffu, (most - ref) * scale > kLag)) {
+            const float now = (most - ref) * scale > kLag ? most : ref, down = ref == -INFINITY ? 0.f : ex2((ref - now) * scale);
+            ref = now;
+            base = ref == -INFINITY ? 0.f : ref * scale;
+            part = mul_two(part, two(down, down));
+            if (s > 0) {                                        // O stands still once the product before this step is done (the one before that is)
+                if (!__all_sync(0xffffffffu, wait_bar(&sh->pv_done[w], (st.pv + s - 1) & 1u, sh, ctl, kErrAttnTile))) return;
+                tc_fence_after();
 #pragma unroll 1
-            for (int i = 0; i < kDim; i += 32) {
-                uint32_t o[32];
-                tc_ld32(to + i, o);
-                tc_landed(o);
+                for (int i = 0; i < kDim; i += 16) {            // few registers: scores are waiting in most of them
+                    uint32_t o[16];
+                    tc_ld16(to + i, o);
+                    tc_landed(o);
 #pragma unroll
-                for (int k = 0; k < 32; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * down);
-                tc_st32(to + i, o);
+                    for (int k = 0; k < 16; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * down);
+                    tc_st16(to + i, o);
+                }
             }
         }
-        float part[4] = {0.f, 0.f, 0.f, 0.f};
-        uint32_t p[32];
-#pragma unroll
-        for (int i = 0; i < 32; ++i) {
-            const float e0 = ex2(fmaf(__uint_as_float(r[2 * i]), scale, -base)), e1 = ex2(fmaf(__uint_as_float(r[2 * i + 1]), scale, -base));
-            part[(2 * i) & 3] += e0;
-            part[(2 * i + 1) & 3] += e1;
-            p[i] = Elem<T>::pack(e0, e1);
+        const bool more = s + 1 < n;
+        exps(lo, 0);
+        if (more) {
+            if (!ready(s + 1)) return;
+            tc_ld32(scores(s + 1), lo);
         }
-        tc_st32(ts, p);
+        exps(hi, 16);
+        if (more) tc_ld32(scores(s + 1) + 32, hi);
+        tc_st32(scores(s), p);
         tc_wait_st();
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(&sh->p_full[w][s & 1]);
-        sum += (part[0] + part[1]) + (part[2] + part[3]);
+        if (more) {                                             // here and not where they are used: registers may be moved in between
+            tc_landed(lo);
+            tc_pin(hi);
+        }
     }
+    const float2 sums = of_two(part);
+    const float sum = sums.x + sums.y;
     st.stage = stage0 + stages_of(x);
     st.keys0 += x.steps0;
     if (!x.both) st.keys1 += x.steps1;
@@ -597,21 +692,11 @@ __device__ __forceinline__ void work_tiles(const CacheView &c, const AttnArgs &a
             }
         }
     } else {
-        // Hidden values that are not finite: the group's rows once more by units, which add such values with selects.  Their rings lie
-        // where the group's queries were (a stage each), which nobody reads any more.
-        units.move(my_q + warp * unit_stage_bytes<kDim>(), 1);
-        for (int i = (x.both ? w * (kTile / kUnitRows) : 0) + warp; i < x.groups && i < (x.both ? (w + 1) * (kTile / kUnitRows) : x.groups); i += 4) {
-            Unit u;
-            u.entry = x.entry;
-            u.head = x.head;
-            u.r0 = x.r0 + i * kUnitRows;
-            u.rows = min(kUnitRows, x.rows - i * kUnitRows);
-            u.from = x.from;
-            u.first = (pos0 - x.from) / kBlock;
-            u.last = min(u.first + n * (kStep / kBlock), (x.end - x.from + kBlock - 1) / kBlock);
-            u.slot = direct ? -1 : x.slot0 + i * x.step + (x.half == 2 ? w : 0);
-            run_unit<T, kDim, 2>(c, a, map_k, map_v, sh, ctl, units, u);
-        }
+        // Hidden values that are not finite: the group's rows once more.
+        const TileItem copy = x;                                // the call wants addresses: not those of what the loop keeps in registers
+        Ring ring_copy = units;
+        redo_rows<T, kDim>(c, a, map_k, map_v, sh, ctl, my_q, ring_copy, copy, w, warp, pos0, n);
+        units = ring_copy;
         if (!group_meet(sh, ctl, st, w)) return;                // the next queries may come
     }
     tc_fence_before();
