@@ -36,6 +36,26 @@ __device__ __forceinline__ int claim(Ctl *ctl, const AttnShared *sh, int which, 
     return t < (unsigned long long)total ? (int)t : -1;
 }
 
+// A ticket for a warp.  Without tiles all warps come here at once, and where nothing can stop a launch its tickets begin at zero: the
+// first round is dealt by the warp's number (spread over the SMs), which saves the wait for a counter, 0.7 us; `dealt`: bit per counter.
+template <bool kPreemptible>
+__device__ __forceinline__ int warp_claim(Ctl *ctl, const AttnShared *sh, int which, int total, uint32_t &dealt) {
+    const bool deal = !kPreemptible && sh->tiles == 0;
+    const int warps = (int)gridDim.x * kWorkers;
+    if (deal && !(dealt >> which & 1u)) {
+        dealt |= 1u << which;
+        const int t = (int)(threadIdx.x >> 5) * (int)gridDim.x + (int)blockIdx.x;
+        return t < total && *(const volatile uint32_t *)&sh->abort == 0u ? t : -1;
+    }
+    if (deal && total <= warps) return -1;
+    int t = -1;
+    if ((threadIdx.x & 31) == 0) {
+        t = claim<kPreemptible>(ctl, sh, which, deal ? total - warps : total);
+        if (deal && t >= 0) t += warps;
+    }
+    return __shfl_sync(0xffffffffu, t, 0);
+}
+
 // An item from the loader; all lanes of a warp, or the issuing thread alone.
 __device__ __forceinline__ int next_item(AttnShared *sh, Ctl *ctl, uint32_t &seen) {
     const uint32_t slot = seen % kSched;
@@ -45,27 +65,26 @@ __device__ __forceinline__ int next_item(AttnShared *sh, Ctl *ctl, uint32_t &see
 }
 
 // Some CTAs begin with tiles (tensor pipe), the others with units (HBM), so that both are busy; each goes on with the rest.
-template <class T, int kDim, bool kPreemptible>
+template <class T, int kDim, bool kPreemptible, bool kTiles>
 __device__ __forceinline__ void workers(Ctl *ctl, const CUtensorMap *map_k, const CUtensorMap *map_v, const CacheView &c, const AttnArgs &a,
                                         AttnShared *sh, unsigned char *smem) {
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const bool tiles = sh->tiles > 0, tiles_first = (int)blockIdx.x < sh->tile_ctas;
+    const bool tiles = kTiles && sh->tiles > 0, tiles_first = tiles && (int)blockIdx.x < sh->tile_ctas;
     unsigned char *const unit_ring = smem + (size_t)warp * kUnitStages * unit_stage_bytes<kDim>();
     Ring ring{unit_ring, sh->full[warp], kUnitStages, 0u, 0u, 0u, 0u};
     unsigned long long done = 0;
+    uint32_t dealt = 0;
     for (int phase = 0; phase < 2; ++phase) {
         if ((phase == 0) != tiles_first) {
-            if (sh->units > 0)
-                while (true) {
-                    int ticket = -1;
-                    if (lane == 0) ticket = claim<kPreemptible>(ctl, sh, kUnitTickets, sh->units);
-                    ticket = __shfl_sync(0xffffffffu, ticket, 0);
-                    if (ticket < 0) break;
-                    unit_ticket<T, kDim>(c, a, map_k, map_v, sh, ctl, ring, ticket);
-                    done += lane == 0;
-                }
+            while (sh->units > 0) {
+                const int ticket = warp_claim<kPreemptible>(ctl, sh, kUnitTickets, sh->units, dealt);
+                if (ticket < 0) break;
+                unit_ticket<T, kDim>(c, a, map_k, map_v, sh, ctl, ring, ticket);
+                done += lane == 0;
+            }
             if (tiles && !tiles_first) __syncthreads();      // the units' rings lie where the tiles will: the loader waits here too
-        } else if (tiles) {
+        } else if constexpr (kTiles) {
+            if (!tiles) continue;
             WorkState st = {};
             uint32_t seen = 0;
             while (true) {
@@ -88,9 +107,7 @@ __device__ __forceinline__ void workers(Ctl *ctl, const CUtensorMap *map_k, cons
     }
     // Without anything to do there is one merge of nothing, so that the call has a ticket to complete.
     while (true) {
-        int ticket = -1;
-        if (lane == 0) ticket = claim<kPreemptible>(ctl, sh, kMergeTickets, sh->merges);
-        ticket = __shfl_sync(0xffffffffu, ticket, 0);
+        const int ticket = warp_claim<kPreemptible>(ctl, sh, kMergeTickets, sh->merges, dealt);
         if (ticket < 0) break;
         run_merge<T, kDim>(c, a, sh, ctl, ticket);
         done += lane == 0;
@@ -161,13 +178,13 @@ __device__ __forceinline__ void helpers(Ctl *ctl, const CUtensorMap *page_k, con
     __syncwarp();
 }
 
-template <class T, int kDim, bool kPreemptible>
+template <class T, int kDim, bool kPreemptible, bool kTiles>
 __device__ __forceinline__ void work_off(Ctl *ctl, const CUtensorMap *map_k, const CUtensorMap *map_v, const CUtensorMap *page_k, const CUtensorMap *page_v,
                                          const CacheView &c, const AttnArgs &a, AttnShared *sh, unsigned char *smem) {
     const int warp = threadIdx.x >> 5;
     make_plan(c, a, sh);
     const int merges = max(sh->merges, sh->tiles + sh->units == 0 ? 1 : 0);
-    const bool tiles = sh->tiles > 0;
+    const bool tiles = kTiles && sh->tiles > 0;
     if (threadIdx.x == 0) {
         // Never zero: a task that was stopped before any CTA got here must not look complete.
         *(volatile unsigned long long *)&ctl->total = (unsigned long long)sh->tiles + sh->units + merges;       // the same from every CTA
@@ -180,9 +197,12 @@ __device__ __forceinline__ void work_off(Ctl *ctl, const CUtensorMap *map_k, con
     __syncthreads();
     tc_fence_after();
     if (threadIdx.x == 0) sh->merges = merges;
-    if (warp < kWorkers) {
+    if constexpr (!kTiles) {
+        workers<T, kDim, kPreemptible, false>(ctl, map_k, map_v, c, a, sh, smem);
+        return;
+    } else if (warp < kWorkers) {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" :: "n"(kWorkerRegs));
-        workers<T, kDim, kPreemptible>(ctl, map_k, map_v, c, a, sh, smem);
+        workers<T, kDim, kPreemptible, true>(ctl, map_k, map_v, c, a, sh, smem);
     } else {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" :: "n"(kHelperRegs));
         helpers<T, kDim, kPreemptible>(ctl, page_k, page_v, c, a, sh, smem);
@@ -194,8 +214,10 @@ __device__ __forceinline__ void work_off(Ctl *ctl, const CUtensorMap *map_k, con
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" :: "r"(*(volatile uint32_t *)&sh->tmem), "r"(kAttnTmemCols) : "memory");
 }
 
-template <class T, int kDim, bool kPreemptible>
-__global__ void __launch_bounds__(kAttnThreads, 1)
+// kTiles: the call may have tiles.  The form without them is what calls run whose sequences have one query each and no prefix: eight warps
+// instead of twelve, and registers for units alone.
+template <class T, int kDim, bool kPreemptible, bool kTiles>
+__global__ void __launch_bounds__(kTiles ? kAttnThreads : kUnitThreads, 1)
 attention_kernel(Ctl *ctl, const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
                  const __grid_constant__ CUtensorMap page_k, const __grid_constant__ CUtensorMap page_v,
                  const __grid_constant__ CacheView c, const __grid_constant__ AttnArgs a, unsigned long long launch_no) {
@@ -227,7 +249,7 @@ attention_kernel(Ctl *ctl, const __grid_constant__ CUtensorMap map_k, const __gr
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     }
     __syncthreads();
-    if (sh->stop == 0u) work_off<T, kDim, kPreemptible>(ctl, &map_k, &map_v, &page_k, &page_v, c, a, sh, smem);
+    if (sh->stop == 0u) work_off<T, kDim, kPreemptible, kTiles>(ctl, &map_k, &map_v, &page_k, &page_v, c, a, sh, smem);
     __syncthreads();
     if (threadIdx.x == 0) sh->last = cta_leave(ctl, sh->done) ? 1u : 0u;
     __syncthreads();
@@ -236,7 +258,7 @@ attention_kernel(Ctl *ctl, const __grid_constant__ CUtensorMap map_k, const __gr
     const bool task = ctl->mailbox != nullptr;
     const bool whole = *(volatile unsigned long long *)&ctl->tiles_done >= *(volatile unsigned long long *)&ctl->total;
     if (whole || !task)
-        for (uint32_t i = threadIdx.x; i < (a.n + 1) * c.heads; i += kAttnThreads) a.counters[i] = 0;
+        for (uint32_t i = threadIdx.x; i < (a.n + 1) * c.heads; i += blockDim.x) a.counters[i] = 0;
     __threadfence();
     __syncthreads();
     if (threadIdx.x == 0) {
@@ -249,9 +271,13 @@ attention_kernel(Ctl *ctl, const __grid_constant__ CUtensorMap map_k, const __gr
 // ---- host side -------------------------------------------------------------------------------------------------
 template <class T, int kDim>
 static cudaError_t prepare_one() {
-    cudaError_t e = cudaFuncSetAttribute(attention_kernel<T, kDim, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)attn_smem<kDim>());
-    if (e != cudaSuccess) return e;
-    return cudaFuncSetAttribute(attention_kernel<T, kDim, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)attn_smem<kDim>());
+    const void *forms[] = {(const void *)attention_kernel<T, kDim, true, true>, (const void *)attention_kernel<T, kDim, true, false>,
+                           (const void *)attention_kernel<T, kDim, false, true>, (const void *)attention_kernel<T, kDim, false, false>};
+    for (const void *f : forms) {
+        const cudaError_t e = cudaFuncSetAttribute(f, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)attn_smem<kDim>());
+        if (e != cudaSuccess) return e;
+    }
+    return cudaSuccess;
 }
 cudaError_t attention_prepare() {
     cudaError_t e = prepare_one<__nv_bfloat16, 128>();
@@ -324,10 +350,13 @@ cudaError_t launch_attention(bool preemptible, Ctl *ctl, const xpkKvCache_st *ca
     const CUtensorMap &mk = *(const CUtensorMap *)cache->map_k, &mv = *(const CUtensorMap *)cache->map_v;
     const CUtensorMap &pk = *(const CUtensorMap *)cache->page_k, &pv = *(const CUtensorMap *)cache->page_v;
     const bool bf16 = cache->d.dtype == XPK_DTYPE_BF16;
-#define XPK_ATTN(T, D)                                                                                                              \
-    do {                                                                                                                            \
-        if (preemptible) attention_kernel<T, D, true><<<grid, kAttnThreads, attn_smem<D>(), st>>>(ctl, mk, mv, pk, pv, c, a, launch_no); \
-        else attention_kernel<T, D, false><<<grid, kAttnThreads, attn_smem<D>(), st>>>(ctl, mk, mv, pk, pv, c, a, launch_no);            \
+    // The host does not know lengths, but a row for each sequence and nothing shared means units only.
+    const bool tiles = a.starts != nullptr || a.shared_len != nullptr || a.group > (uint32_t)kUnitRowsMost;
+#define XPK_ATTN(T, D)                                                                                                                          \
+    do {                                                                                                                                        \
+        auto *f = tiles ? (preemptible ? attention_kernel<T, D, true, true> : attention_kernel<T, D, false, true>)                             \
+                        : (preemptible ? attention_kernel<T, D, true, false> : attention_kernel<T, D, false, false>);                          \
+        f<<<grid, tiles ? kAttnThreads : kUnitThreads, attn_smem<D>(), st>>>(ctl, mk, mv, pk, pv, c, a, launch_no);                             \
     } while (0)
     if (bf16 && c.dim == 128) XPK_ATTN(__nv_bfloat16, 128);
     else if (bf16) XPK_ATTN(__nv_bfloat16, 64);

@@ -7,7 +7,8 @@
 namespace xpk {
 
 constexpr int kWorkers = 8;                                 // warps that run units and merges; two groups of four for tiles
-constexpr int kAttnThreads = (kWorkers + 4) * 32;           // and a third group: one warp loads, one issues MMAs
+constexpr int kUnitThreads = kWorkers * 32;
+constexpr int kAttnThreads = kUnitThreads + 128;            // and a third group for tiles: one warp loads, one issues MMAs
 // Registers: 384 threads are launched with 168 each; the workers, whose rows of scores fill 128, take over what the helpers
 // do not need: 2 * 208 + 88 = 3 * 168.
 constexpr int kWorkerRegs = 208, kHelperRegs = 88;
@@ -27,7 +28,7 @@ constexpr int kShareRows = 64;                              // sequences of more
 constexpr int kMergeRowsMost = 32;
 constexpr int kPageWords = 16;                              // more than the steps that a ring holds
 constexpr int kSched = 2;                                   // items the loader may be ahead
-constexpr float kTileUs = 1.6f;                             // measured time of a tile of 256 rows at head_dim 128
+constexpr float kTileUs = 2.6f;                             // measured time of a tile of 256 rows at head_dim 128
 constexpr uint32_t kErrAttnLoad  = 0x70000001u;
 constexpr uint32_t kErrAttnMerge = 0x70000002u;
 constexpr uint32_t kErrAttnTile  = 0x70000003u;
@@ -175,12 +176,12 @@ __device__ __forceinline__ unsigned long long warp_sum(unsigned long long v) {
 // Every CTA works the same cut out of the same arrays, a thread per sequence.
 __device__ __forceinline__ void make_plan(const CacheView &c, const AttnArgs &a, AttnShared *sh) {
     const uint32_t tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    constexpr uint32_t kWarps = kAttnThreads / 32;
+    const uint32_t threads = blockDim.x, warps = threads / 32;
     int shared = a.shared_len ? max(*a.shared_len, 0) & ~(int)(c.page - 1) : 0;
     if (tid < 4) sh->sums[tid] = 0;
     if (tid == 4) sh->first_sharing = 0xffffffffu;
     __syncthreads();
-    for (uint32_t base = 0; base < a.n; base += kAttnThreads) {              // whole warps: ballots below
+    for (uint32_t base = 0; base < a.n; base += threads) {              // whole warps: ballots below
         const uint32_t i = base + tid;
         bool with = false;
         if (i < a.n) {
@@ -213,7 +214,7 @@ __device__ __forceinline__ void make_plan(const CacheView &c, const AttnArgs &a,
         }
         __syncthreads();
         unsigned long long blocks = 0, tiles = 0, rows = 0;
-        for (uint32_t i = tid; i < a.n; i += kAttnThreads) {
+        for (uint32_t i = tid; i < a.n; i += threads) {
             const SeqPlan p = sh->plan[i];
             if (p.seq < 0) continue;
             const int own = p.len - own_from(sh, (int)i);
@@ -250,7 +251,7 @@ __device__ __forceinline__ void make_plan(const CacheView &c, const AttnArgs &a,
         int4 carry = make_int4(0, 0, 0, 0);
         if (shared > 0) carry.y = row_tiles(sh->pre_rows) * (int)c.heads * tile_runs(sh, shared);
         const int pre_items = carry.y;
-        for (uint32_t base = 0; base < a.n; base += kAttnThreads) {
+        for (uint32_t base = 0; base < a.n; base += threads) {
             const uint32_t i = base + tid;
             int4 v = make_int4(0, 0, 0, 0);                                  // units, tile items, results, sharing rows
             if (i < a.n && sh->plan[i].seq >= 0) {
@@ -274,7 +275,7 @@ __device__ __forceinline__ void make_plan(const CacheView &c, const AttnArgs &a,
             if (lane == 31) sh->warp_sums[warp] = s;
             __syncthreads();
             int4 before = carry;
-            for (uint32_t w = 0; w < kWarps && base + w * 32 < a.n; ++w) {
+            for (uint32_t w = 0; w < warps && base + w * 32 < a.n; ++w) {
                 const int4 y = sh->warp_sums[w];
                 if (w < warp) { before.x += y.x; before.y += y.y; before.z += y.z; before.w += y.w; }
                 carry.x += y.x; carry.y += y.y; carry.z += y.z; carry.w += y.w;

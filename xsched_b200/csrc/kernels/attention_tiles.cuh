@@ -82,6 +82,11 @@ __device__ __forceinline__ void tc_landed(uint32_t (&r)[N]) {
 }
 __device__ __forceinline__ void tc_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
+__device__ __forceinline__ float max_three(float a, float b, float c) {
+    float d;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
+}
 // Two fp32 operations an instruction.
 __device__ __forceinline__ uint64_t two(float a, float b) {
     uint64_t x;
@@ -576,7 +581,7 @@ __device__ __forceinline__ void work_tiles(const CacheView &c, const AttnArgs &a
 #pragma unroll
         for (int i = 0; i < 32; i += 4)
 #pragma unroll
-            for (int k = 0; k < 4; ++k) top[k] = fmaxf(fmaxf(top[k], __uint_as_float(lo[i + k])), __uint_as_float(hi[i + k]));
+            for (int k = 0; k < 4; ++k) top[k] = max_three(top[k], __uint_as_float(lo[i + k]), __uint_as_float(hi[i + k]));
         const float most = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
         // (-inf) - (-inf) is no reason to move.
         if (__any_sync(0xffffffffu, (most - ref) * scale > kLag)) {

@@ -5,9 +5,9 @@
 //   (a, b) <- (a cos t - b sin t, b cos t + a sin t),   t = position * inv_freq[j]
 //
 // HBM-bound: every element is read once and written once (2 + 2 bytes), 12 KB in and 12 KB out per row at 32 + 2 * 8
-// heads of 128.  One CTA takes a row: a thread holds 16 bytes (8 elements) of a head at a time, so a head is 16 (8) lanes
-// of one warp and the mean is four (three) shuffles.  All of a thread's loads are issued first; under them the row's
-// rotary / 2 angles are computed once and shared by all heads through shared memory.
+// heads of 128.  A thread holds 16 bytes (8 elements) of a head at a time, so a head is 16 (8) lanes of one warp and the mean
+// is four (three) shuffles.  A CTA takes one row, or four where there are many; its places, and its rotary / 2 angles a row, which
+// all heads share through shared memory, are worked out under the loads of the first words.
 //
 // Angles: a position of 900,000 times a frequency of 1 leaves an fp32 angle with an error of 0.03; so the product and its
 // reduction to [-pi, pi] are fp64 and only the remainder is rounded (2e-7) before sincosf.  The pairs (j, j + rotary / 2)
@@ -45,56 +45,93 @@ __device__ __forceinline__ uint4 close8(const float (&f)[8]) {
     return make_uint4(Pair<T>::close(f[0], f[1]), Pair<T>::close(f[2], f[3]), Pair<T>::close(f[4], f[5]), Pair<T>::close(f[6], f[7]));
 }
 
-// The entry of `starts` [n + 1] that row r belongs to: the last one that starts at or before it (-1: none).
-__device__ __forceinline__ int entry_of(const int32_t *starts, uint32_t n, int r) {
-    int lo = -1, hi = (int)n;                                   // starts[lo] <= r < starts[hi]
+// The entry of `starts` [n + 1] that row r belongs to: the last one that starts at or before it (-1: none); the whole warp.
+// Each look narrows it down by 32 with one load a lane: a halving search would wait for memory five times as often.
+__device__ __forceinline__ int entry_of(const int32_t *starts, int n, int r) {
+    const int lane = threadIdx.x & 31;
+    int lo = -1, hi = n;                                        // starts[lo] <= r < starts[hi]
     while (hi - lo > 1) {
-        const int mid = (lo + hi) >> 1;
-        if (starts[mid] <= r) lo = mid; else hi = mid;
+        const int step = (hi - lo + 31) / 32, at = lo + (lane + 1) * step;
+        const bool below = at < hi && starts[at] <= r;
+        const int got = __popc(__ballot_sync(0xffffffffu, below));
+        const int from = lo + got * step;
+        hi = min(hi, from + step);
+        lo = from;
     }
     return lo >= 0 && r < starts[lo + 1] ? lo : -1;
 }
 
-// kLanes = head_dim / 8 threads hold a head.
-template <class T, int kLanes>
-__global__ void __launch_bounds__(kAppendThreads) kv_append_kernel(CacheView c, xpkKvAppendArgs a) {
+struct RowPlace {
+    long long pos;              // of the row in its sequence, -1: nothing to do
+    int page;                   // -1: not there
+};
+
+// kLanes = head_dim / 8 threads hold a head; kRows consecutive rows a CTA: where they go and their angles are found side by
+// side, under the loads of the first row's words.
+template <class T, int kLanes, int kRows>
+__global__ void __launch_bounds__(kAppendThreads, 4) kv_append_kernel(CacheView c, xpkKvAppendArgs a) {
     constexpr int kDim = kLanes * 8;
     constexpr int kAhead = 3;                                   // 16-byte words a thread holds at once
-    __shared__ float2 s_turn[kDim / 2];                         // cos, sin
+    __shared__ float2 s_turn[kRows][kDim / 2];                  // cos, sin
+    __shared__ RowPlace s_place[kRows];
     const uint32_t words = (a.q_heads + 2 * c.heads) * kLanes;  // 16-byte words of a row
     const int half = (int)a.rotary / 2;
-    for (uint32_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
+    const uint32_t row0 = blockIdx.x * kRows;
+    auto word = [&](uint32_t row, uint32_t w) {
         const uint4 *x = reinterpret_cast<const uint4 *>(static_cast<const T *>(a.qkv) + (size_t)row * a.qkv_stride);
-        uint4 got[kAhead];
+        return w < words && row < a.rows ? __ldcs(x + w) : make_uint4(0, 0, 0, 0);
+    };
+    uint4 got[kAhead];
 #pragma unroll
-        for (int k = 0; k < kAhead; ++k) {
-            const uint32_t w = threadIdx.x + k * kAppendThreads;
-            got[k] = w < words ? x[w] : make_uint4(0, 0, 0, 0);
+    for (int k = 0; k < kAhead; ++k) got[k] = word(row0, threadIdx.x + k * kAppendThreads);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    if (warp < kRows) {
+        const uint32_t row = row0 + warp;
+        RowPlace at{-1, -1};
+        if (row < a.rows) {
+            const int entry = a.starts ? entry_of(a.starts, (int)a.n, (int)row) : (row < a.n ? (int)row : -1);
+            if (entry >= 0) {
+                const int seq = a.seqs ? a.seqs[entry] : entry;
+                const int len = held_by(c, seq);
+                const long long pos = a.starts ? (long long)len - a.starts[entry + 1] + (long long)row : (long long)len - 1;
+                if (len >= 0 && pos >= 0) {
+                    at.pos = pos;
+                    at.page = c.table[(size_t)seq * c.width + (pos >> c.page_shift)];
+                    if ((uint32_t)at.page >= c.pages) at.page = -1;
+                }
+            }
         }
-        const int entry = a.starts ? entry_of(a.starts, a.n, (int)row) : (row < a.n ? (int)row : -1);
-        if (entry < 0) continue;                                // the same for the whole CTA, as is what follows
-        const int seq = a.seqs ? a.seqs[entry] : entry;
-        const int len = held_by(c, seq);
-        const long long pos = a.starts ? (long long)len - a.starts[entry + 1] + (long long)row : (long long)len - 1;
-        if (len < 0 || pos < 0) continue;
-        const int page = c.table[(size_t)seq * c.width + (pos >> c.page_shift)];
-        const bool there = page >= 0 && (uint32_t)page < c.pages;
-        __syncthreads();                                        // s_turn of the row before has been read
-        for (int j = threadIdx.x; j < half; j += kAppendThreads) {
-            const double t = (double)pos * a.inv_freq[j];
-            const double turns = rint(t * 0.15915494309189533577);
-            // 2 pi in two parts: turns times the first is exact enough to leave the angle's own rounding as the only error.
-            const double left = fma(-turns, 2.4492935982947064e-16, fma(-turns, 6.283185307179586232, t));
-            float sn, cs;
-            sincosf((float)left, &sn, &cs);
-            s_turn[j] = make_float2(cs, sn);
-        }
-        __syncthreads();
+        if (lane == 0) s_place[warp] = at;
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < half * kRows; i += kAppendThreads) {
+        const int r = i / half, j = i - r * half;
+        const long long pos = s_place[r].pos;
+        if (pos < 0) continue;
+        const double t = (double)pos * a.inv_freq[j];
+        const double turns = rint(t * 0.15915494309189533577);
+        // 2 pi in two parts: turns times the first is exact enough to leave the angle's own rounding as the only error.
+        const double left = fma(-turns, 2.4492935982947064e-16, fma(-turns, 6.283185307179586232, t));
+        float sn, cs;
+        sincosf((float)left, &sn, &cs);
+        s_turn[r][j] = make_float2(cs, sn);
+    }
+    __syncthreads();
+#pragma unroll 1
+    for (int r = 0; r < kRows; ++r) {
+        const uint32_t row = row0 + r;
+        const RowPlace at = s_place[r];
+        const bool there = at.page >= 0;
         for (uint32_t base = 0; base < words; base += kAhead * kAppendThreads) {
+            uint4 next[kAhead];                                 // the words after these: of the row, or of the row behind it
+            const bool last = base + kAhead * kAppendThreads >= words;
+#pragma unroll
+            for (int k = 0; k < kAhead; ++k)
+                next[k] = last && r + 1 == kRows ? make_uint4(0, 0, 0, 0)
+                                                 : word(last ? row + 1 : row, (last ? 0 : base + kAhead * kAppendThreads) + threadIdx.x + k * kAppendThreads);
 #pragma unroll
             for (int k = 0; k < kAhead; ++k) {
                 const uint32_t w = base + threadIdx.x + k * kAppendThreads;
-                if (base != 0) got[k] = w < words ? x[w] : make_uint4(0, 0, 0, 0);
                 const uint32_t head = w / kLanes;
                 const int in = (int)(w % kLanes) * 8;           // first element of this thread's eight
                 const bool is_q = head < a.q_heads, is_v = head >= a.q_heads + c.heads;
@@ -103,23 +140,23 @@ __global__ void __launch_bounds__(kAppendThreads) kv_append_kernel(CacheView c, 
                 float f[8];
                 open8<T>(got[k], f);
                 const void *weight = is_q ? a.q_weight : a.k_weight;
-                float sum = 0.f;
-#pragma unroll
-                for (int i = 0; i < 8; ++i) sum = fmaf(f[i], f[i], sum);
-#pragma unroll
-                for (int d = kLanes / 2; d > 0; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
                 if (weight != nullptr) {
+                    float sum = 0.f;
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) sum = fmaf(f[i], f[i], sum);
+#pragma unroll
+                    for (int d = kLanes / 2; d > 0; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
                     float g[8];
                     open8<T>(*reinterpret_cast<const uint4 *>(static_cast<const T *>(weight) + in), g);
-                    const float r = rsqrtf(sum * (1.f / kDim) + a.eps);
+                    const float s = rsqrtf(sum * (1.f / kDim) + a.eps);
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) f[i] = f[i] * r * g[i];
+                    for (int i = 0; i < 8; ++i) f[i] = f[i] * s * g[i];
                 }
                 if (a.interleaved) {
                     if (in < (int)a.rotary) {
 #pragma unroll
                         for (int i = 0; i < 8; i += 2) {
-                            const float2 t = s_turn[(in + i) >> 1];
+                            const float2 t = s_turn[r][(in + i) >> 1];
                             const float u = f[i], v = f[i + 1];
                             f[i] = u * t.x - v * t.y;
                             f[i + 1] = v * t.x + u * t.y;
@@ -128,41 +165,47 @@ __global__ void __launch_bounds__(kAppendThreads) kv_append_kernel(CacheView c, 
                 } else if (half != 0) {
                     // The partner's eight elements: `half / 8` lanes up for the first half, down for the second.
                     const bool lower = in < half;
-                    const int partner = (int)(threadIdx.x & 31) + (lower ? half / 8 : -(half / 8));
-                    const int from = in < (int)a.rotary ? partner : (int)(threadIdx.x & 31);
+                    const int partner = lane + (lower ? half / 8 : -(half / 8));
+                    const int from = in < (int)a.rotary ? partner : lane;
 #pragma unroll
                     for (int i = 0; i < 8; ++i) {
                         const float other = __shfl_sync(0xffffffffu, f[i], from);
                         if (in < (int)a.rotary) {
-                            const float2 t = s_turn[(lower ? in : in - half) + i];
+                            const float2 t = s_turn[r][(lower ? in : in - half) + i];
                             f[i] = lower ? f[i] * t.x - other * t.y : f[i] * t.x + other * t.y;
                         }
                     }
                 }
-                if (w >= words) continue;
+                if (w >= words || at.pos < 0) continue;         // the latter the same for the whole CTA
                 if (!is_v) out = close8<T>(f);
                 if (is_q) {
-                    *reinterpret_cast<uint4 *>(static_cast<T *>(a.q) + (size_t)row * a.q_stride + (size_t)head * kDim + in) = out;
+                    __stcs(reinterpret_cast<uint4 *>(static_cast<T *>(a.q) + (size_t)row * a.q_stride + (size_t)head * kDim + in), out);
                 } else if (there) {
                     const uint32_t h = is_v ? head - a.q_heads - c.heads : head - a.q_heads;
                     T *pool = reinterpret_cast<T *>(is_v ? c.v : c.k);
-                    const size_t slab = ((size_t)a.layer * c.pages + page) * c.heads + h;
-                    *reinterpret_cast<uint4 *>(pool + ((slab << c.page_shift) + (size_t)(pos & (c.page - 1))) * kDim + in) = out;
+                    const size_t slab = ((size_t)a.layer * c.pages + at.page) * c.heads + h;
+                    *reinterpret_cast<uint4 *>(pool + ((slab << c.page_shift) + (size_t)(at.pos & (c.page - 1))) * kDim + in) = out;
                 }
             }
+#pragma unroll
+            for (int k = 0; k < kAhead; ++k) got[k] = next[k];
         }
     }
 }
 
+template <class T, int kLanes>
+static void launch_rows(const CacheView &c, const xpkKvAppendArgs &a, int sms, cudaStream_t st) {
+    // Four rows a CTA share one search, one set of look-ups and fill the threads with angles, where there are rows enough for every
+    // SM to have several CTAs of them (273 MB of prompts: 104 -> 55 us); fewer rows are spread, one a CTA.
+    if (a.rows >= (uint32_t)sms * 8) kv_append_kernel<T, kLanes, 4><<<(a.rows + 3) / 4, kAppendThreads, 0, st>>>(c, a);
+    else kv_append_kernel<T, kLanes, 1><<<a.rows, kAppendThreads, 0, st>>>(c, a);
+}
+
 cudaError_t launch_kv_append(const CacheView &c, const xpkKvAppendArgs &a, bool bf16, int sms, cudaStream_t st) {
-    const int grid = (int)min((unsigned long long)a.rows, (unsigned long long)sms * 64);
-    if (bf16) {
-        if (c.dim == 128) kv_append_kernel<__nv_bfloat16, 16><<<grid, kAppendThreads, 0, st>>>(c, a);
-        else kv_append_kernel<__nv_bfloat16, 8><<<grid, kAppendThreads, 0, st>>>(c, a);
-    } else {
-        if (c.dim == 128) kv_append_kernel<__half, 16><<<grid, kAppendThreads, 0, st>>>(c, a);
-        else kv_append_kernel<__half, 8><<<grid, kAppendThreads, 0, st>>>(c, a);
-    }
+    if (bf16 && c.dim == 128) launch_rows<__nv_bfloat16, 16>(c, a, sms, st);
+    else if (bf16) launch_rows<__nv_bfloat16, 8>(c, a, sms, st);
+    else if (c.dim == 128) launch_rows<__half, 16>(c, a, sms, st);
+    else launch_rows<__half, 8>(c, a, sms, st);
     return cudaGetLastError();
 }
 

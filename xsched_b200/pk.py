@@ -265,9 +265,10 @@ class Task:
 
 def _rows(what: str, x, width: int):
     """(rows, elements between rows) of a tensor whose trailing dimensions, `width` elements in all, are dense."""
-    rows = x.shape[0]
+    shape = x.shape
+    rows = shape[0]
     if x.numel() != rows * width:
-        raise ValueError(f"{what}: {tuple(x.shape)} is not [rows] of {width} elements")
+        raise ValueError(f"{what}: {tuple(shape)} is not [rows] of {width} elements")
     if x.is_contiguous():
         return rows, 0
     inner = 1
@@ -301,7 +302,8 @@ class KvCache:
             if not x.is_contiguous() or x.device != k.device or not x.is_cuda:
                 raise ValueError(f"{name} is contiguous and on the same CUDA device as k")
         self.k, self.v, self.page_table, self.lens, self.refs = k, v, page_table, lens, refs
-        self.device, self.dtype, self.heads, self.dim = k.device, k.dtype, heads, dim
+        self.device, self.dtype, self.heads, self.dim, self.seqs = k.device, k.dtype, heads, dim, lens.numel()
+        self._int32 = lens.dtype
         self.handle = None
         d = KvCacheDesc(k.data_ptr(), v.data_ptr(), page_table.data_ptr(), lens.data_ptr(), refs.data_ptr(), dtype, layers, pages, heads, page, dim,
                         page_table.shape[0], page_table.shape[1])
@@ -320,7 +322,7 @@ class KvCache:
     def _ints(self, what: str, x):
         if x is None:
             return None
-        if str(x.dtype) != "torch.int32" or not x.is_contiguous() or x.device != self.device:
+        if x.dtype is not self._int32 or not x.is_contiguous() or x.device != self.device:
             raise ValueError(f"{what} is a contiguous int32 tensor on {self.device}")
         return x.data_ptr()
 
@@ -332,7 +334,7 @@ class KvCache:
     def _data(self, what: str, x):
         if x is None:
             return None
-        if x.dtype != self.dtype or x.device != self.device:
+        if x.dtype is not self.dtype or x.device != self.device:
             raise ValueError(f"{what} is {self.dtype} on {self.device}, got {x.dtype} on {x.device}")
         return x.data_ptr()
 
@@ -342,8 +344,8 @@ class KvCache:
             raise ValueError(f"starts has {starts.numel()} entries for {n} sequences: one more is wanted")
         if starts is None and n != rows:
             raise ValueError(f"{rows} rows for {n} sequences: without `starts` each has one")
-        if seqs is None and n > self.lens.numel():
-            raise ValueError(f"{n} sequences, the cache has {self.lens.numel()}")
+        if seqs is None and n > self.seqs:
+            raise ValueError(f"{n} sequences, the cache has {self.seqs}")
         return n
 
     # -- pages --------------------------------------------------------------------------
@@ -384,7 +386,7 @@ class KvCache:
         for name, w in (("q_weight", q_weight), ("k_weight", k_weight)):
             if w is not None and (w.numel() != self.dim or not w.is_contiguous()):
                 raise ValueError(f"{name} has {self.dim} elements")
-        if inv_freq is not None and (str(inv_freq.dtype) != "torch.float64" or not inv_freq.is_contiguous() or inv_freq.device != self.device):
+        if inv_freq is not None and (inv_freq.element_size() != 8 or not inv_freq.is_floating_point() or not inv_freq.is_contiguous() or inv_freq.device != self.device):
             raise ValueError("inv_freq is a contiguous float64 tensor on the cache's device")
         a = KvAppendArgs(self._data("q", q), self._data("qkv", qkv), q_stride, qkv_stride, self._ints("seqs", seqs), self._ints("starts", starts),
                          self._data("q_weight", q_weight), self._data("k_weight", k_weight), None if inv_freq is None else inv_freq.data_ptr(), eps,
