@@ -363,11 +363,11 @@ __device__ __forceinline__ void run_merge(const CacheView &c, const AttnArgs &a,
             const float w = ml.x == -INFINITY && ml.y == 0.f ? -1.f : ex2(ml.x - base);
             if (!(w < 0.f)) sum = fmaf(w, ml.y, sum);
             const int here = min(32, all - b);
-            // Eight results in flight: one after another they would cost an L2 round trip each.
-            for (int i0 = 0; i0 < here; i0 += 8) {
-                float x[8][kVec], wi[8];
+            // Sixteen results in flight: one after another they would cost an L2 round trip each.
+            for (int i0 = 0; i0 < here; i0 += 16) {
+                float x[16][kVec], wi[16];
 #pragma unroll
-                for (int u = 0; u < 8; ++u) {
+                for (int u = 0; u < 16; ++u) {
                     const int i = min(i0 + u, 31);
                     wi[u] = __shfl_sync(0xffffffffu, w, i);
                     const bool real = i0 + u < here && !(wi[u] < 0.f);
@@ -382,7 +382,7 @@ __device__ __forceinline__ void run_merge(const CacheView &c, const AttnArgs &a,
                     }
                 }
 #pragma unroll
-                for (int u = 0; u < 8; ++u)
+                for (int u = 0; u < 16; ++u)
 #pragma unroll
                     for (int v = 0; v < kVec; ++v) acc[v] = fmaf(wi[u], x[u][v], acc[v]);
             }

@@ -69,10 +69,10 @@ struct RowPlace {
 // kLanes = head_dim / 8 threads hold a head; kRows consecutive rows a CTA: where they go and their angles are found side by
 // side, under the loads of the first row's words.
 template <class T, int kLanes, int kRows>
-__global__ void __launch_bounds__(kAppendThreads, 4) kv_append_kernel(CacheView c, xpkKvAppendArgs a) {
+__global__ void __launch_bounds__(kAppendThreads, 3) kv_append_kernel(CacheView c, xpkKvAppendArgs a) {
     constexpr int kDim = kLanes * 8;
     constexpr int kAhead = 3;                                   // 16-byte words a thread holds at once
-    __shared__ float2 s_turn[kRows][kDim / 2];                  // cos, sin
+    __shared__ float2 s_turn[kRows][kDim / 2];                  // cos, sin; a thread's are kept apart, so that lanes read side by side
     __shared__ RowPlace s_place[kRows];
     const uint32_t words = (a.q_heads + 2 * c.heads) * kLanes;  // 16-byte words of a row
     const int half = (int)a.rotary / 2;
@@ -114,14 +114,32 @@ __global__ void __launch_bounds__(kAppendThreads, 4) kv_append_kernel(CacheView 
         const double left = fma(-turns, 2.4492935982947064e-16, fma(-turns, 6.283185307179586232, t));
         float sn, cs;
         sincosf((float)left, &sn, &cs);
-        s_turn[r][j] = make_float2(cs, sn);
+        // A thread turns eight elements: pairs 8 t .. 8 t + 7 of the halves, or the four neighbours' pairs 4 t .. 4 t + 3.
+        s_turn[r][a.interleaved ? (j & 3) * (half / 4) + j / 4 : (j & 7) * (half / 8) + j / 8] = make_float2(cs, sn);
     }
     __syncthreads();
+    // 256 threads are whole heads: a thread's eight elements lie at the same place of every head it gets, so its turns and its
+    // weights are fetched once.
+    const int in = (int)(threadIdx.x % kLanes) * 8;
+    const bool turned = in < (int)a.rotary, lower = in < half;
+    uint4 wq = make_uint4(0, 0, 0, 0), wk = wq;
+    if (a.q_weight != nullptr) {
+        wq = *reinterpret_cast<const uint4 *>(static_cast<const T *>(a.q_weight) + in);
+        wk = *reinterpret_cast<const uint4 *>(static_cast<const T *>(a.k_weight) + in);
+    }
+    const int partner = !turned || a.interleaved ? lane : lane + (lower ? half / 8 : -(half / 8));
+    const float sign = lower ? -1.f : 1.f;
 #pragma unroll 1
     for (int r = 0; r < kRows; ++r) {
         const uint32_t row = row0 + r;
         const RowPlace at = s_place[r];
         const bool there = at.page >= 0;
+        float2 turn[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            turn[i] = make_float2(1.f, 0.f);
+            if (turned) turn[i] = a.interleaved ? s_turn[r][(i >> 1) * (half / 4) + in / 8] : s_turn[r][i * (half / 8) + (lower ? in : in - half) / 8];
+        }
         for (uint32_t base = 0; base < words; base += kAhead * kAppendThreads) {
             uint4 next[kAhead];                                 // the words after these: of the row, or of the row behind it
             const bool last = base + kAhead * kAppendThreads >= words;
@@ -133,47 +151,36 @@ __global__ void __launch_bounds__(kAppendThreads, 4) kv_append_kernel(CacheView 
             for (int k = 0; k < kAhead; ++k) {
                 const uint32_t w = base + threadIdx.x + k * kAppendThreads;
                 const uint32_t head = w / kLanes;
-                const int in = (int)(w % kLanes) * 8;           // first element of this thread's eight
                 const bool is_q = head < a.q_heads, is_v = head >= a.q_heads + c.heads;
                 uint4 out = got[k];
                 // Every lane takes part in the shuffles; lanes of values and of nothing throw their results away.
                 float f[8];
                 open8<T>(got[k], f);
-                const void *weight = is_q ? a.q_weight : a.k_weight;
-                if (weight != nullptr) {
+                if (a.q_weight != nullptr) {
                     float sum = 0.f;
 #pragma unroll
                     for (int i = 0; i < 8; ++i) sum = fmaf(f[i], f[i], sum);
 #pragma unroll
                     for (int d = kLanes / 2; d > 0; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
                     float g[8];
-                    open8<T>(*reinterpret_cast<const uint4 *>(static_cast<const T *>(weight) + in), g);
+                    open8<T>(is_q ? wq : wk, g);
                     const float s = rsqrtf(sum * (1.f / kDim) + a.eps);
 #pragma unroll
                     for (int i = 0; i < 8; ++i) f[i] = f[i] * s * g[i];
                 }
-                if (a.interleaved) {
-                    if (in < (int)a.rotary) {
+                if (a.interleaved && turned) {
 #pragma unroll
-                        for (int i = 0; i < 8; i += 2) {
-                            const float2 t = s_turn[r][(in + i) >> 1];
-                            const float u = f[i], v = f[i + 1];
-                            f[i] = u * t.x - v * t.y;
-                            f[i + 1] = v * t.x + u * t.y;
-                        }
+                    for (int i = 0; i < 8; i += 2) {
+                        const float u = f[i], v = f[i + 1];
+                        f[i] = u * turn[i].x - v * turn[i].y;
+                        f[i + 1] = v * turn[i].x + u * turn[i].y;
                     }
-                } else if (half != 0) {
-                    // The partner's eight elements: `half / 8` lanes up for the first half, down for the second.
-                    const bool lower = in < half;
-                    const int partner = lane + (lower ? half / 8 : -(half / 8));
-                    const int from = in < (int)a.rotary ? partner : lane;
+                } else if (!a.interleaved && half != 0) {
+                    // The partner's eight elements are `half / 8` lanes up for the first half, down for the second.
 #pragma unroll
                     for (int i = 0; i < 8; ++i) {
-                        const float other = __shfl_sync(0xffffffffu, f[i], from);
-                        if (in < (int)a.rotary) {
-                            const float2 t = s_turn[r][(lower ? in : in - half) + i];
-                            f[i] = lower ? f[i] * t.x - other * t.y : f[i] * t.x + other * t.y;
-                        }
+                        const float other = __shfl_sync(0xffffffffu, f[i], partner);
+                        if (turned) f[i] = f[i] * turn[i].x + sign * other * turn[i].y;
                     }
                 }
                 if (w >= words || at.pos < 0) continue;         // the latter the same for the whole CTA
