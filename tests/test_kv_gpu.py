@@ -645,3 +645,47 @@ def test_refusals(pk, kv):
     torch.cuda.synchronize()
     assert not bool(out.any()) and not bool(scratch.any())
     c.destroy()
+
+
+# ------------------------------------------------------------------------------------------------- in the decode workload
+def test_paged_decode_step_equals_attention_over_each_request_by_itself(pk, kv):
+    """PagedCache of the decode workload: forks of one prompt that grow at different times, one of them ends and another takes its
+    place; each step's attention against the definition, and nothing is left of the pages at the end."""
+    from xsched_b200 import llama_decode as ld
+    g = _gen(30)
+    c = ld.PagedCache(g, 2, 100, 4, 40, torch.device("cuda"))
+    live, table = [], lambda: c.cache.page_table.cpu().numpy()
+    for step in range(30):
+        if step in (0, 3, 20):
+            new = {0: [1, 2], 3: [3], 20: [2, 4]}[step]
+            c.start(_ints(new))
+            live += new
+        if step == 15:
+            c.stop(_ints([2]))
+            live.remove(2)
+            c.compact()
+        seqs = _ints(live)
+        c.extend(seqs)
+        for layer in range(2):
+            qkv = _normal(g, torch.bfloat16, len(live), (ld.NQ + 2 * ld.NKV) * ld.HD)
+            out = c.step(layer, qkv, seqs)
+            if step % 7 == 1:
+                lens = c.cache.lens.cpu().numpy()
+                want, size, big = kv.attention(c.q[:len(live)], c.k[layer], c.v[layer], table(), lens, live, list(range(len(live) + 1)), float(np.float32(ld.HD ** -0.5)))
+                bound = 2.0 ** -8 * want.abs() + 1.004 * (2.0 ** -8 + 2 * ld.HD * 2.0 ** -24 * big + 300 * 2.0 ** -24) * size + 2.0 ** -126
+                assert float(((out.double() - want).abs() / bound).max()) <= 1.0
+    assert c.cache.lens.tolist() == [100, 130, 110, 127, 110]
+    c.stop(_ints([1, 2, 3, 4]))
+    assert c.cache.refs.sum().item() == 2 and c.cache.lens.tolist() == [100, 0, 0, 0, 0]
+    c.cache.destroy()
+
+
+def test_decode_workload_runs_paged():
+    import json
+    import subprocess
+    import sys
+    r = subprocess.run([sys.executable, "-m", "xsched_b200.llama_decode", "--requests", "6", "--tokens", "5", "--rate", "200", "--layers", "2", "--kv", "300",
+                        "--batched", "--max-batch", "4", "--paged"], capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0, r.stderr[-2000:]
+    line = json.loads(r.stdout.strip().splitlines()[-1])
+    assert line["mode"] == "batched, paged" and line["requests"] == 6 and line["tokens"] == 30

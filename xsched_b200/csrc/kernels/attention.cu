@@ -299,10 +299,10 @@ AttnScratch attention_scratch(const CacheView &c, uint32_t sms, uint32_t rows, u
     // slots a result, two halves).  With a prefix every sharing sequence leaves some: one per key head if it is of one row
     // group (all are where each has a single query of up to 16 heads), at most eight; the prefix itself 16 per item.
     const size_t group = q_heads / c.heads, most = std::min<size_t>(n, rows);
-    const size_t base = 2 * (size_t)kUnitWaves * sms * kWorkers + 64 * (size_t)sms;
+    const size_t base = 2 * (size_t)kUnitWaves * sms * kWorkers + 128 * (size_t)sms;
     const size_t own = c.heads * most * (rows <= n && group <= kUnitRows ? 1 : 8);
     const size_t pre_rows = std::min<size_t>((size_t)rows * group, most * kShareRows);
-    const size_t pre = 16 * (c.heads * ((pre_rows + kItemRows - 1) / kItemRows) + 2 * (size_t)sms);
+    const size_t pre = 16 * (c.heads * ((pre_rows + kItemRows - 1) / kItemRows) + 4 * (size_t)sms);
     // More than 2^16 slots (1/2 GB at 128) are not worth a prefix: the kernel does without it if they do not suffice.
     s.part_slots = (uint32_t)(base + std::min<size_t>(own + pre, 1u << 16));
     s.ctl = 0;

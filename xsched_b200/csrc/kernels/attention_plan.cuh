@@ -23,7 +23,7 @@ constexpr int kItemRows = 2 * kTile;
 constexpr int kStep = 64;                                   // positions per product; tiles are counted in pairs of steps
 constexpr int kRing = 8;                                    // stages of the tile ring; a stage holds a step's keys or values
 constexpr int kMinRun = 4;                                  // blocks: a run shorter than 64 positions costs more to merge than it spreads
-constexpr int kMinTiles = 2;                                // tiles: one for each group of workers
+constexpr int kMinTiles = 4;                                // tiles: two for each group of workers
 constexpr int kShareRows = 64;                              // sequences of more rows fill tiles by themselves
 constexpr int kMergeRowsMost = 32;
 constexpr int kPageWords = 16;                              // more than the steps that a ring holds
@@ -157,7 +157,11 @@ __device__ __forceinline__ int row_tiles(long long rows) { return (int)((rows + 
 // With at most 128 rows the two groups of workers take half of a run's tiles each, and leave a result each.
 __device__ __forceinline__ int halves(long long rows) { return rows <= kTile ? 2 : 1; }
 __device__ __forceinline__ int chunks(int positions, int each, int run) { return max(1, ((positions + each - 1) / each + run - 1) / run); }
-__device__ __forceinline__ int tile_runs(const AttnShared *sh, int positions) { return chunks(positions, kTile, sh->tile_run); }
+__device__ __forceinline__ int tiles_of(int positions) { return (positions + kTile - 1) / kTile; }
+// Runs of about tile_run tiles, equally long: the last item to end should not be a short one's neighbour.
+__device__ __forceinline__ int tile_runs(const AttnShared *sh, int positions) {
+    return max(1, (tiles_of(positions) + sh->tile_run / 2) / sh->tile_run);
+}
 // Results that are left for each row by a sequence's own runs, and by the prefix.
 __device__ __forceinline__ int runs_of(const AttnShared *sh, uint32_t group, int i) {
     const SeqPlan &p = sh->plan[i];
@@ -239,12 +243,15 @@ __device__ __forceinline__ void make_plan(const CacheView &c, const AttnArgs &a,
         const unsigned long long target = (unsigned long long)a.sms * kWorkers * kUnitWaves;
         if (tid == 0) {
             sh->run = max(kMinRun, (int)min((blocks + target - 1) / target, 0x7fffffffull / kBlock));
-            sh->tile_run = max(kMinTiles, (int)min((tiles + a.sms - 1) / a.sms, 0x7fffffffull / kTile));
             sh->pre_rows = (int)rows;
             // CTAs are dealt to tiles and units by the time each kind takes: a tile of 256 rows about kTileUs of an SM, a block
-            // 64 bytes an element over the SM's share of HBM (44 GB/s): 0.19 us at 128.
+            // 64 bytes an element over the SM's share of HBM (44 GB/s): 0.19 us at 128.  Those that begin with tiles get one item each: two rounds of shorter
+            // ones left more results to merge than they balanced (256 sequences on 16384: 259 against 224 us).
             const float tile_us = kTileUs * (float)tiles * ((float)c.dim / 128.f), block_us = 0.0015f * (float)c.dim * (float)blocks;
-            sh->tile_ctas = tiles == 0 ? 0 : blocks == 0 ? 0x7fffffff : max(1, (int)((float)gridDim.x * tile_us / (tile_us + block_us) + 0.5f));
+            const float share = tiles == 0 ? 0.f : blocks == 0 ? 1.f : tile_us / (tile_us + block_us);
+            const unsigned long long items = max((unsigned long long)((float)a.sms * share), 1ull);
+            sh->tile_run = max(kMinTiles, (int)min((tiles + items - 1) / items, 0x7fffffffull / kTile));
+            sh->tile_ctas = tiles == 0 ? 0 : max(1, (int)((float)gridDim.x * share + 0.5f));
         }
         __syncthreads();
         // Tickets and partial results before each sequence: a scan in each warp, then over the warps.
@@ -299,6 +306,7 @@ __device__ __forceinline__ void make_plan(const CacheView &c, const AttnArgs &a,
             sh->units = carry.x;
             sh->tiles = carry.y;
             sh->pre_tiles = pre_items;
+            if (carry.y > 0 && carry.y < (int)gridDim.x && carry.x > 0) sh->tile_ctas = carry.y;          // one each: a second item would be the last to end
             sh->pre_part0 = carry.z;
             const uint32_t out_rows = a.rows * a.q_heads;
             int per = 1;

@@ -187,7 +187,7 @@ __device__ __forceinline__ TileItem tile_ticket(const AttnArgs &a, const CacheVi
         const SeqPlan &p = sh->plan[x.entry];
         most = min(max(p.len - p.t + (x.r0 + x.rows - 1) / (int)a.group + 1 - x.from, 0), own);
     }
-    const int first = run * sh->tile_run, last = min(first + sh->tile_run, (most + kTile - 1) / kTile), count = max(last - first, 0);
+    const int each = (tiles_of(own) + runs - 1) / runs, first = run * each, last = min(first + each, tiles_of(most)), count = max(last - first, 0);
     x.both = x.half == 1 && x.rows > kTile;
     const int head_tiles = x.half == 2 ? (count + 1) / 2 : count;              // of the first group where each takes a half
     x.pos0 = x.from + first * kTile;

@@ -348,8 +348,11 @@ __device__ __forceinline__ void run_merge(const CacheView &c, const AttnArgs &a,
         const size_t in_p = (size_t)(cr % kUnitRows), in_o = (size_t)(r % kUnitRows);
         const int all = np + runs;
         auto at = [&](int i) { return i < np ? (slot_p + i) * kUnitRows + in_p : (slot_o + (i - np)) * kUnitRows + in_o; };
-        float top = -INFINITY;
-        for (int i = lane; i < all; i += 32) top = fmaxf(top, __ldcg(&a.part_ml[at(i)]).x);
+        // Lane l keeps the maximum and sum of result l: most rows have no more than 32.
+        float2 first = make_float2(-INFINITY, 0.f);
+        if (lane < all) first = __ldcg(&a.part_ml[at(lane)]);
+        float top = first.x;
+        for (int i = lane + 32; i < all; i += 32) top = fmaxf(top, __ldcg(&a.part_ml[at(i)]).x);
 #pragma unroll
         for (int d = 16; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
         const float base = top == -INFINITY ? 0.f : top;
@@ -357,8 +360,8 @@ __device__ __forceinline__ void run_merge(const CacheView &c, const AttnArgs &a,
 #pragma unroll
         for (int v = 0; v < kVec; ++v) acc[v] = 0.f;
         for (int b = 0; b < all; b += 32) {
-            float2 ml = make_float2(-INFINITY, 0.f);
-            if (b + lane < all) ml = __ldcg(&a.part_ml[at(b + lane)]);
+            float2 ml = first;
+            if (b > 0) ml = b + lane < all ? __ldcg(&a.part_ml[at(b + lane)]) : make_float2(-INFINITY, 0.f);
             // A run in which the row saw nothing may have left its sum unwritten: it is passed over (weight -1).
             const float w = ml.x == -INFINITY && ml.y == 0.f ? -1.f : ex2(ml.x - base);
             if (!(w < 0.f)) sum = fmaf(w, ml.y, sum);

@@ -16,6 +16,12 @@ for all of them, every request is still a batch-1 client with its own KV cache o
 tokens).  That is what makes the configured 10 requests/s servable at all: one request at a time needs ~0.7 s of
 decode per request, seven times more than one GPU has at that rate.  A token's latency is then the duration of the
 step that produced it, counted once per request that was in the step.
+
+With --paged (and --batched) the caches are one paged cache (xsched_b200.pk.KvCache) and its operators take the place of
+the cache writes, the attention and the slot moves above: every request is a fork of one prompt of --kv positions, whose
+pages all share; each token extends it by a position (the first one copies the shared last page), is rotated by its position
+and written by `append`, and attends through `attention`, which reads the shared positions once for the whole batch.  A
+request that is done frees its pages; the pool is compacted while nothing is in flight.
 """
 from __future__ import annotations
 
@@ -34,6 +40,9 @@ def pct(v, p):
     return v[min(len(v) - 1, int(p * (len(v) - 1) + 0.5))] if v else float("nan")
 
 
+PAGE = 64
+
+
 class Layer:
     def __init__(self, g, kv_len, dev, slots=1):
         def w(o, i):
@@ -44,6 +53,8 @@ class Layer:
         self.w_down = w(H, FFN)
         self.n1 = torch.ones(H, device=dev, dtype=torch.bfloat16)
         self.n2 = torch.ones(H, device=dev, dtype=torch.bfloat16)
+        if slots == 0:                                    # the cache is elsewhere (--paged)
+            return
         self.k = (torch.randn(1, NKV, kv_len, HD, device=dev, generator=g) * 0.5).to(torch.bfloat16).expand(slots, -1, -1, -1).contiguous()
         self.v = (torch.randn(1, NKV, kv_len, HD, device=dev, generator=g) * 0.5).to(torch.bfloat16).expand(slots, -1, -1, -1).contiguous()
 
@@ -76,10 +87,73 @@ class Layer:
         g_, u_ = gu.split([FFN, FFN], dim=-1)
         return x + (torch.nn.functional.silu(g_) * u_) @ self.w_down.T
 
+    def paged(self, x, index, kv, seqs):
+        """The same for n requests in a paged cache: x [n, H], seqs [n] = their slots, already extended by this token."""
+        n = x.shape[0]
+        h = torch.nn.functional.rms_norm(x, (H,), self.n1, 1e-5)
+        att = kv.step(index, h @ self.wqkv.T, seqs)
+        x = x + att.view(n, NQ * HD) @ self.wo.T
+        h = torch.nn.functional.rms_norm(x, (H,), self.n2, 1e-5)
+        gu = h @ self.w_gate_up.T
+        g_, u_ = gu.split([FFN, FFN], dim=-1)
+        return x + (torch.nn.functional.silu(g_) * u_) @ self.w_down.T
+
     def move_slot(self, src, dst):
         """The request in cache slot `src` continues in slot `dst` (slots in use stay contiguous)."""
         self.k[dst].copy_(self.k[src])
         self.v[dst].copy_(self.v[src])
+
+
+class PagedCache:
+    """One paged cache for all layers: sequence 0 holds the prompt, sequences 1.. are the requests, forks of it."""
+
+    def __init__(self, g, layers, prompt, slots, tokens, dev):
+        from xsched_b200 import pk
+        own = -(-(prompt + tokens) // PAGE) - prompt // PAGE      # pages that a request may need of its own
+        pages, width = -(-prompt // PAGE) + slots * own, -(-(prompt + tokens) // PAGE)
+        self.k = torch.empty(layers, pages, NKV, PAGE, HD, device=dev, dtype=torch.bfloat16)
+        self.v = torch.empty_like(self.k)
+        for pool in (self.k, self.v):
+            for layer in pool:
+                layer.copy_(torch.randn(layer.shape, device=dev, generator=g) * 0.5)
+        table = torch.full((1 + slots, width), -1, dtype=torch.int32, device=dev)
+        lens, refs = torch.zeros(1 + slots, dtype=torch.int32, device=dev), torch.zeros(pages, dtype=torch.int32, device=dev)
+        self.cache = pk.KvCache(self.k, self.v, table, lens, refs)
+        self.prompt = torch.zeros(1, dtype=torch.int32, device=dev)
+        self.one = torch.ones(slots, dtype=torch.int32, device=dev)
+        self.shared = torch.full((1,), prompt, dtype=torch.int32, device=dev)
+        self.inv_freq = 500000.0 ** (-torch.arange(0, HD, 2, device=dev, dtype=torch.float64) / HD)
+        self.q, self.out = (torch.empty(slots, NQ, HD, device=dev, dtype=torch.bfloat16) for _ in range(2))
+        self.scratch = torch.zeros(self.cache.attention_scratch_bytes(slots, slots, NQ), dtype=torch.uint8, device=dev)
+        self.cache.extend(self.prompt, self.shared, self._stream())
+        self._settled(self.cache.result(self._stream()))
+
+    @staticmethod
+    def _stream():
+        return torch.cuda.current_stream().cuda_stream
+
+    @staticmethod
+    def _settled(report):
+        if report.missing or report.refused:
+            raise RuntimeError(f"the page pool is too small: {report.missing} pages missing, {report.refused} sequences too long")
+
+    def start(self, seqs):
+        self.cache.fork(self.prompt.expand(seqs.numel()).contiguous(), seqs, self._stream())
+
+    def stop(self, seqs):
+        self.cache.free(seqs, self._stream())
+
+    def extend(self, seqs):
+        self.cache.extend(seqs, self.one[:seqs.numel()], self._stream())
+
+    def compact(self):
+        self.cache.compact(self._stream())
+
+    def step(self, layer, qkv, seqs):
+        n, s = seqs.numel(), self._stream()
+        self.cache.append(self.q[:n], qkv, seqs, s, inv_freq=self.inv_freq, layer=layer)
+        self.cache.attention(self.out[:n], self.q[:n], seqs, s, scratch=self.scratch, shared_len=self.shared, layer=layer)
+        return self.out[:n]
 
 
 def main() -> None:
@@ -95,11 +169,14 @@ def main() -> None:
     ap.add_argument("--samples", default="", help="write every per-token latency (ms, one per line) to this file")
     ap.add_argument("--batched", action="store_true", help="decode the requests in flight together (continuous batching)")
     ap.add_argument("--max-batch", type=int, default=16)
+    ap.add_argument("--paged", action="store_true", help="with --batched: one paged cache, requests are forks of one prompt of --kv positions")
     a = ap.parse_args()
+    if a.paged and not a.batched:
+        ap.error("--paged goes with --batched")
     torch.cuda.set_device(a.device)
     dev = torch.device("cuda", a.device)
     g = torch.Generator(device=dev).manual_seed(a.seed)
-    layers = [Layer(g, a.kv, dev, a.max_batch if a.batched else 1) for _ in range(a.layers)]
+    layers = [Layer(g, a.kv, dev, 0 if a.paged else a.max_batch if a.batched else 1) for _ in range(a.layers)]
     lm_head = (torch.randn(VOCAB, H, device=dev, generator=g) * 0.02).to(torch.bfloat16)
     norm = torch.ones(H, device=dev, dtype=torch.bfloat16)
     torch.cuda.synchronize()
@@ -119,31 +196,54 @@ def main() -> None:
             xb = torch.randn(a.max_batch, H, device=dev, generator=g).to(torch.bfloat16)
             rows_all = torch.arange(a.max_batch, device=dev)
 
-            def bstep(n, pos_list):
-                pos = torch.tensor(pos_list, device=dev)
-                x = xb[:n]
-                for l in layers:
-                    x = l.batched(x, rows_all[:n], pos)
-                xb[:n] = x
+            kv = PagedCache(g, a.layers, a.kv, a.max_batch, a.tokens + 2 * a.max_batch, dev) if a.paged else None
+
+            def logits_of(x):
                 logits = torch.nn.functional.rms_norm(x, (H,), norm, 1e-5) @ lm_head.T
                 return logits.argmax(dim=-1).tolist()      # the device->host read of the step's result
 
+            def bstep(n, pos_list):
+                x = xb[:n]
+                if kv is not None:
+                    seqs = torch.tensor(pos_list, dtype=torch.int32, device=dev)
+                    kv.extend(seqs)
+                    for i, l in enumerate(layers):
+                        x = l.paged(x, i, kv, seqs)
+                else:
+                    pos = torch.tensor(pos_list, device=dev)
+                    for l in layers:
+                        x = l.batched(x, rows_all[:n], pos)
+                xb[:n] = x
+                return logits_of(x)
+
             for n in list(range(1, a.max_batch + 1)) * 2:                      # warm-up: every batch size once picks its kernels
-                bstep(n, [n] * n)
+                if kv is None:
+                    bstep(n, [n] * n)
+                    continue
+                seqs = list(range(1, n + 1))
+                kv.start(torch.tensor(seqs, dtype=torch.int32, device=dev))
+                bstep(n, seqs)
+                kv.stop(torch.tensor(seqs, dtype=torch.int32, device=dev))
             print("READY", flush=True)
             t0 = time.perf_counter()
             arrivals, t = [], t0
             for _ in range(a.requests):
                 t += rng.expovariate(a.rate)
                 arrivals.append(t)
-            active = []                               # [arrival time, tokens done, write position]; index = cache slot
+            active = []                               # [arrival time, tokens done, write position, or the sequence if paged]; index = cache slot
+            free_seqs = list(range(a.max_batch, 0, -1))
             nxt = 0
             while nxt < len(arrivals) or active:
                 now = time.perf_counter()
                 while nxt < len(arrivals) and arrivals[nxt] <= now and len(active) < a.max_batch:
-                    active.append([arrivals[nxt], 0, (nxt * 37) % a.kv])
+                    if kv is not None:
+                        seq = free_seqs.pop()
+                        kv.start(torch.tensor([seq], dtype=torch.int32, device=dev))
+                    active.append([arrivals[nxt], 0, (nxt * 37) % a.kv if kv is None else seq])
                     nxt += 1
                 if not active:
+                    if kv is not None:
+                        kv.compact()                  # nobody waits for a page now
                     time.sleep(max(0.0, arrivals[nxt] - time.perf_counter()))
                     continue
                 n = len(active)
@@ -157,14 +257,18 @@ def main() -> None:
                 while slot < len(active):
                     r = active[slot]
                     r[1] += 1
-                    r[2] = (r[2] + 1) % a.kv
+                    if kv is None:
+                        r[2] = (r[2] + 1) % a.kv
                     if r[1] < a.tokens:
                         slot += 1
                         continue
                     req_ms.append((end - r[0]) * 1e3)
                     last = len(active) - 1
+                    if kv is not None:
+                        kv.stop(torch.tensor([r[2]], dtype=torch.int32, device=dev))
+                        free_seqs.append(r[2])
                     if slot != last:                  # the last slot's request moves into the freed one
-                        for l in layers:
+                        for l in layers if kv is None else ():
                             l.move_slot(last, slot)
                         xb[slot].copy_(xb[last])
                         active[slot] = active[last]
@@ -197,7 +301,7 @@ def main() -> None:
                       "token_p99_ms": round(pct(tok_ms, 0.99), 3), "token_mean_ms": round(sum(tok_ms) / max(1, len(tok_ms)), 3),
                       "request_p50_ms": round(pct(req_ms, 0.5), 2), "request_p99_ms": round(pct(req_ms, 0.99), 2),
                       "weights_gb": round(weights_gb, 2), "kv_gb": round(a.layers * 2 * NKV * a.kv * HD * 2 / 1e9, 3), "rate": a.rate,
-                      "mode": "batched" if a.batched else "one request at a time", "decode_steps": len(batch_sizes) if a.batched else len(tok_ms),
+                      "mode": "batched, paged" if a.paged else "batched" if a.batched else "one request at a time", "decode_steps": len(batch_sizes) if a.batched else len(tok_ms),
                       "mean_batch": round(sum(batch_sizes) / max(1, len(batch_sizes)), 2) if a.batched else 1.0,
                       "deadline_ms": a.deadline_ms, "deadline_missed": missed, "deadline_miss_rate": round(missed / max(1, len(tok_ms)), 5)}))
 
