@@ -216,7 +216,7 @@ xpkResult xpkSortNoAlloc(int32_t *keys, int32_t *tmp, uint64_t n, void *stream);
  *   lens        [seqs] positions that a sequence holds (0 = the slot is free)
  *   refs        [pages] how many table entries name a page (0 = the page is free)
  *
- * page_size is 16, 32, 64 or 128, head_dim 64 or 128.  The three integer arrays live on the device, and every call
+ * page_size is 16, 32, 64 or 128, head_dim 64 or 128, table_width * page_size at most 2^30.  The three integer arrays live on the device, and every call
  * reads what they hold when its kernels run, so a loop can be captured once and replayed while lengths grow.  Page ids
  * and sequence ids are checked by the kernels: a sequence outside [0, seqs) is padding and is passed over, a page
  * outside [0, pages) is treated as not there (never read, never written).
@@ -240,6 +240,7 @@ typedef struct {
 
 /* Checks the description and allocates the handle's workspace (12 bytes per page and 8 KB on the device). */
 xpkResult xpkKvCacheCreate(xpkKvCache_t *cache, const xpkKvCacheDesc *desc);
+/* Tasks created on the cache go first. */
 xpkResult xpkKvCacheDestroy(xpkKvCache_t cache);
 
 /* At most this many entries in the lists of fork and extend. */
@@ -313,7 +314,8 @@ xpkResult xpkKvAppend(xpkKvCache_t cache, const xpkKvAppendArgs *args, void *str
  * padded sequences and behind starts[n] stay as they are.
  *
  * `scratch`: xpkAttentionScratchBytes bytes, 256-byte aligned, zeroed once before its first use; a call leaves it ready
- * for the next.  Calls that may overlap on the GPU (other streams, other captured graphs) need scratch of their own.
+ * for the next one on the same cache, whatever its sizes.  Calls that may overlap on the GPU (other streams, other captured graphs)
+ * need scratch of their own.
  * A call that was refused wrote nothing.  n <= XPK_ATTENTION_MAX_SEQS. */
 #define XPK_ATTENTION_MAX_SEQS 1024
 typedef struct {

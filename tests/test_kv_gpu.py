@@ -382,6 +382,30 @@ def test_padding_repeated_sequences_and_scratch_that_is_used_again(pk, kv):
     c.destroy()
 
 
+def test_scratch_serves_calls_of_other_sizes_in_turn(pk, kv):
+    """What one call leaves in its partial results must not be where a later, larger call counts."""
+    lens = [700 + 13 * i for i in range(40)]
+    c = _filled(pk, lens, 16, 4, 64, torch.bfloat16)
+    scratch = torch.zeros(c.attention_scratch_bytes(40 * 9, 40, 16), dtype=torch.uint8, device="cuda")
+    for seqs, count in (([39], 1), (list(range(40)), 1), ([0, 1], 9), (list(range(40)), 9), ([5, 6, 7], 1), (list(range(40)), 1)):
+        starts = [count * i for i in range(len(seqs) + 1)]
+        q = _normal(_gen(31), torch.bfloat16, starts[-1], 16, 64)
+        out = _attend(pk, c, q, _ints(seqs), None if count == 1 else _ints(starts), len(seqs), scratch=scratch)
+        _check(kv, c, q, out, seqs, starts)
+    c.destroy()
+
+
+@pytest.mark.parametrize("shared", [None, 64])
+def test_as_many_sequences_as_a_call_takes(pk, kv, shared):
+    lens = [65 + (i * 37) % 200 for i in range(pk.ATTENTION_MAX_SEQS)]
+    c = _filled(pk, lens, 64, 1, 64, torch.float16)
+    _share(c, lens, 64)
+    q = _normal(_gen(32), torch.float16, len(lens), 2, 64)
+    out = _attend(pk, c, q, None, None, len(lens), shared=shared)
+    _check(kv, c, q, out, list(range(len(lens))), list(range(len(lens) + 1)))
+    c.destroy()
+
+
 def test_missing_pages_are_left_out(pk, kv):
     lens = [300, 64, 20]
     c = _filled(pk, lens, 16, 2, 128, torch.float16)

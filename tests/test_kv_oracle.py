@@ -83,6 +83,7 @@ def _desc(pk, **change):
     (dict(dtype=0), 4), (dict(dtype=3), 4), (dict(page_size=8), 4), (dict(page_size=48), 4), (dict(head_dim=96), 4), (dict(head_dim=256), 4),
     (dict(k=0x10008), 2), (dict(v=0x20002), 2), (dict(refs=0x50002), 2),
     (dict(layers=1 << 16, pages=1 << 16), 7), (dict(pages=0xFFFFFFFF), 7),
+    (dict(table_width=(1 << 26) + 1), 7), (dict(kv_heads=65537), 7),
 ])
 def test_cache_descriptions_that_are_refused(pk, change, code):
     h = ctypes.c_void_p(77)

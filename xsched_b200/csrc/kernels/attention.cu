@@ -307,7 +307,8 @@ AttnScratch attention_scratch(const CacheView &c, uint32_t sms, uint32_t rows, u
     s.part_slots = (uint32_t)(base + std::min<size_t>(own + pre, 1u << 16));
     s.ctl = 0;
     s.counters = up(sizeof(Ctl));
-    s.ml = s.counters + up(((size_t)n + 1) * c.heads * 4);
+    // As many counters as any call needs: what has to be zero lies at the same place for all calls that use the scratch in turn.
+    s.ml = s.counters + up((size_t)(XPK_ATTENTION_MAX_SEQS + 1) * c.heads * 4);
     s.part = s.ml + up((size_t)s.part_slots * kUnitRows * sizeof(float2));
     s.bytes = s.part + (size_t)s.part_slots * kUnitRows * c.dim * sizeof(float);
     return s;

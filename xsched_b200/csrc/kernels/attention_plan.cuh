@@ -58,7 +58,7 @@ struct AttnShared {
     int part0[XPK_ATTENTION_MAX_SEQS];                      // its first partial result, -1: written directly
     int pre0[XPK_ATTENTION_MAX_SEQS];                       // rows of sharing sequences before it
     uint32_t share[XPK_ATTENTION_MAX_SEQS / 32];            // which sequences share
-    unsigned long long sums[4];                             // blocks, tiles, sharing rows, sharing sequences
+    unsigned long long sums[5];                             // blocks, tiles, sharing rows, sharing sequences, row groups of units
     int4 warp_sums[kAttnThreads / 32];
     uint32_t first_sharing;
     // tile pipeline
@@ -182,8 +182,8 @@ __device__ __forceinline__ void make_plan(const CacheView &c, const AttnArgs &a,
     const uint32_t tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const uint32_t threads = blockDim.x, warps = threads / 32;
     int shared = a.shared_len ? max(*a.shared_len, 0) & ~(int)(c.page - 1) : 0;
-    if (tid < 4) sh->sums[tid] = 0;
-    if (tid == 4) sh->first_sharing = 0xffffffffu;
+    if (tid < 5) sh->sums[tid] = 0;
+    if (tid == 5) sh->first_sharing = 0xffffffffu;
     __syncthreads();
     for (uint32_t base = 0; base < a.n; base += threads) {              // whole warps: ballots below
         const uint32_t i = base + tid;
@@ -217,30 +217,38 @@ __device__ __forceinline__ void make_plan(const CacheView &c, const AttnArgs &a,
             sh->shared_seq = shared > 0 ? sh->plan[sh->first_sharing].seq : -1;
         }
         __syncthreads();
-        unsigned long long blocks = 0, tiles = 0, rows = 0;
+        unsigned long long blocks = 0, tiles = 0, rows = 0, groups = 0;
         for (uint32_t i = tid; i < a.n; i += threads) {
             const SeqPlan p = sh->plan[i];
             if (p.seq < 0) continue;
             const int own = p.len - own_from(sh, (int)i);
             if (by_tiles(p, a.group)) tiles += (unsigned long long)((own + kTile - 1) / kTile) * row_tiles(rows_of(p, a.group));
-            else blocks += (unsigned long long)((own + kBlock - 1) / kBlock) * row_groups(rows_of(p, a.group));
+            else {
+                blocks += (unsigned long long)((own + kBlock - 1) / kBlock) * row_groups(rows_of(p, a.group));
+                groups += row_groups(rows_of(p, a.group));
+            }
             if (shares(sh, (int)i)) rows += (unsigned long long)rows_of(p, a.group);
         }
         if (warp * 32 < a.n) {
             blocks = warp_sum(blocks);
             tiles = warp_sum(tiles);
             rows = warp_sum(rows);
+            groups = warp_sum(groups);
             if (lane == 0) {
                 atomicAdd(&sh->sums[0], blocks);
                 atomicAdd(&sh->sums[1], tiles);
                 atomicAdd(&sh->sums[2], rows);
+                atomicAdd(&sh->sums[4], groups);
             }
         }
         __syncthreads();
         blocks = sh->sums[0] * c.heads;
         rows = sh->sums[2];
         tiles = (sh->sums[1] + (unsigned long long)((shared + kTile - 1) / kTile) * row_tiles((long long)rows)) * c.heads;
-        const unsigned long long target = (unsigned long long)a.sms * kWorkers * kUnitWaves;
+        // Units come out at work / run and about half a unit more for each row group; a few more than kUnitWaves rounds of all warps
+        // would be a round of their own.
+        const unsigned long long waves = (unsigned long long)a.sms * kWorkers * kUnitWaves, halves_of = sh->sums[4] * c.heads / 2;
+        const unsigned long long target = max(waves - min(waves, halves_of), waves / 4);
         if (tid == 0) {
             sh->run = max(kMinRun, (int)min((blocks + target - 1) / target, 0x7fffffffull / kBlock));
             sh->pre_rows = (int)rows;
@@ -299,7 +307,7 @@ __device__ __forceinline__ void make_plan(const CacheView &c, const AttnArgs &a,
         if (shared > 0) parts += row_groups(sh->pre_rows) * (int)c.heads * pre_runs(sh);
         if (shared > 0 && parts > (int)a.part_slots) {                        // the same for all threads
             shared = 0;
-            if (tid < 3) sh->sums[tid] = 0;
+            if (tid < 3 || tid == 4) sh->sums[tid] = 0;
             continue;
         }
         if (tid == 0) {

@@ -283,8 +283,9 @@ __device__ __forceinline__ void unit_ticket(const CacheView &c, const AttnArgs &
     w.r0 = local / runs % groups * kUnitRows;
     w.rows = (int)min(rows_of(p, a.group) - w.r0, (long long)kUnitRows);
     w.from = own_from(sh, lo);
-    w.first = run * sh->run;
-    w.last = min(w.first + sh->run, (p.len - w.from + kBlock - 1) / kBlock);
+    const int blocks = (p.len - w.from + kBlock - 1) / kBlock, each = (blocks + runs - 1) / runs;      // equally long
+    w.first = run * each;
+    w.last = min(w.first + each, blocks);
     w.slot = sh->part0[lo] < 0 ? -1 : sh->part0[lo] + local;
     if (w.rows > 8) run_unit<T, kDim, 2>(c, a, map_k, map_v, sh, ctl, ring, w);
     else run_unit<T, kDim, 1>(c, a, map_k, map_v, sh, ctl, ring, w);

@@ -109,8 +109,9 @@ xpkResult xpkKvCacheCreate(xpkKvCache_t *cache, const xpkKvCacheDesc *desc) {
     if (d.dtype != XPK_DTYPE_BF16 && d.dtype != XPK_DTYPE_F16) return XPK_ERR_NOT_SUPPORTED;
     if (d.page_size != 16 && d.page_size != 32 && d.page_size != 64 && d.page_size != 128) return XPK_ERR_NOT_SUPPORTED;
     if (d.head_dim != 64 && d.head_dim != 128) return XPK_ERR_NOT_SUPPORTED;
-    // Page ids, pages over all layers and the units of a page over all layers are 32-bit signed in the kernels.
+    // Positions, page ids, pages over all layers and the units of a page over all layers are 32-bit signed in the kernels.
     if (d.pages > 0x7ffffff0u || (uint64_t)d.layers * d.pages > 0x7fffffffull || d.seqs > 0x7fffffffu || d.kv_heads > 65536u ||
+        (uint64_t)d.table_width * d.page_size > (1ull << 30) ||
         (uint64_t)d.layers * d.kv_heads * d.page_size * d.head_dim * 4 / 2048 > 0x7fffffffull) return XPK_ERR_TOO_LARGE;
     if (!aligned16(d.k) || !aligned16(d.v)) return XPK_ERR_ALIGNMENT;
     if (!aligned4(d.page_table) || !aligned4(d.lens) || !aligned4(d.refs)) return XPK_ERR_ALIGNMENT;
