@@ -259,13 +259,13 @@ attention_kernel(Ctl *ctl, const __grid_constant__ CUtensorMap map_k, const __gr
     const bool whole = *(volatile unsigned long long *)&ctl->tiles_done >= *(volatile unsigned long long *)&ctl->total;
     if (whole || !task)
         for (uint32_t i = threadIdx.x; i < (a.n + 1) * c.heads; i += blockDim.x) a.counters[i] = 0;
+    if (!task) {                                           // a call without a task keeps nothing, not even an error
+        if (threadIdx.x < kCtlResetBytes / 8) reinterpret_cast<unsigned long long *>(ctl)[threadIdx.x] = 0;
+        return;
+    }
     __threadfence();
     __syncthreads();
-    if (threadIdx.x == 0) {
-        cta_fold(ctl, launch_no);
-        if (!task)                                         // a call without a task keeps nothing, not even an error
-            for (unsigned i = 0; i < kCtlResetBytes / 8; ++i) reinterpret_cast<unsigned long long *>(ctl)[i] = 0;
-    }
+    if (threadIdx.x == 0) cta_fold(ctl, launch_no);
 }
 
 // ---- host side -------------------------------------------------------------------------------------------------
