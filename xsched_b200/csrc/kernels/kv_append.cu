@@ -128,7 +128,6 @@ __global__ void __launch_bounds__(kAppendThreads, 3) kv_append_kernel(CacheView 
         wk = *reinterpret_cast<const uint4 *>(static_cast<const T *>(a.k_weight) + in);
     }
     const int partner = !turned || a.interleaved ? lane : lane + (lower ? half / 8 : -(half / 8));
-    const float sign = lower ? -1.f : 1.f;
 #pragma unroll 1
     for (int r = 0; r < kRows; ++r) {
         const uint32_t row = row0 + r;
@@ -139,7 +138,12 @@ __global__ void __launch_bounds__(kAppendThreads, 3) kv_append_kernel(CacheView 
         for (int i = 0; i < 8; ++i) {
             turn[i] = make_float2(1.f, 0.f);
             if (turned) turn[i] = a.interleaved ? s_turn[r][(i >> 1) * (half / 4) + in / 8] : s_turn[r][i * (half / 8) + (lower ? in : in - half) / 8];
+            if (lower && !a.interleaved) turn[i].y = -turn[i].y;
         }
+        T *const q_row = static_cast<T *>(a.q) + (size_t)row * a.q_stride + in;
+        const size_t slot = (((((size_t)a.layer * c.pages + max(at.page, 0)) * c.heads) << c.page_shift) + (size_t)(max(at.pos, 0ll) & (c.page - 1))) * kDim + in;
+        T *const k_row = reinterpret_cast<T *>(c.k) + slot, *const v_row = reinterpret_cast<T *>(c.v) + slot;
+        const uint32_t head_step = (uint32_t)kDim << c.page_shift;       // elements between heads of a page
         for (uint32_t base = 0; base < words; base += kAhead * kAppendThreads) {
             uint4 next[kAhead];                                 // the words after these: of the row, or of the row behind it
             const bool last = base + kAhead * kAppendThreads >= words;
@@ -153,46 +157,46 @@ __global__ void __launch_bounds__(kAppendThreads, 3) kv_append_kernel(CacheView 
                 const uint32_t head = w / kLanes;
                 const bool is_q = head < a.q_heads, is_v = head >= a.q_heads + c.heads;
                 uint4 out = got[k];
-                // Every lane takes part in the shuffles; lanes of values and of nothing throw their results away.
-                float f[8];
-                open8<T>(got[k], f);
-                if (a.q_weight != nullptr) {
-                    float sum = 0.f;
+                // Every lane of a warp with a query or a key takes part in the shuffles; its other lanes throw their results away.
+                if (__any_sync(0xffffffffu, !is_v)) {
+                    float f[8];
+                    open8<T>(out, f);
+                    if (a.q_weight != nullptr) {
+                        float sum = 0.f;
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) sum = fmaf(f[i], f[i], sum);
+                        for (int i = 0; i < 8; ++i) sum = fmaf(f[i], f[i], sum);
 #pragma unroll
-                    for (int d = kLanes / 2; d > 0; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
-                    float g[8];
-                    open8<T>(is_q ? wq : wk, g);
-                    const float s = rsqrtf(sum * (1.f / kDim) + a.eps);
+                        for (int d = kLanes / 2; d > 0; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+                        float g[8];
+                        open8<T>(is_q ? wq : wk, g);
+                        const float s = rsqrtf(sum * (1.f / kDim) + a.eps);
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) f[i] = f[i] * s * g[i];
-                }
-                if (a.interleaved && turned) {
-#pragma unroll
-                    for (int i = 0; i < 8; i += 2) {
-                        const float u = f[i], v = f[i + 1];
-                        f[i] = u * turn[i].x - v * turn[i].y;
-                        f[i + 1] = v * turn[i].x + u * turn[i].y;
+                        for (int i = 0; i < 8; ++i) f[i] = f[i] * s * g[i];
                     }
-                } else if (!a.interleaved && half != 0) {
-                    // The partner's eight elements are `half / 8` lanes up for the first half, down for the second.
+                    if (a.interleaved) {
+                        if (turned) {
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) {
-                        const float other = __shfl_sync(0xffffffffu, f[i], partner);
-                        if (turned) f[i] = f[i] * turn[i].x + sign * other * turn[i].y;
+                            for (int i = 0; i < 8; i += 2) {
+                                const float u = f[i], v = f[i + 1];
+                                f[i] = u * turn[i].x - v * turn[i].y;
+                                f[i + 1] = v * turn[i].x + u * turn[i].y;
+                            }
+                        }
+                    } else if (half != 0) {
+                        // The partner's eight elements are `half / 8` lanes up for the first half, down for the second.
+                        float other[8];
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) other[i] = __shfl_sync(0xffffffffu, f[i], partner);
+                        if (turned) {
+#pragma unroll
+                            for (int i = 0; i < 8; ++i) f[i] = fmaf(f[i], turn[i].x, other[i] * turn[i].y);
+                        }
                     }
+                    if (!is_v) out = close8<T>(f);
                 }
                 if (w >= words || at.pos < 0) continue;         // the latter the same for the whole CTA
-                if (!is_v) out = close8<T>(f);
-                if (is_q) {
-                    __stcs(reinterpret_cast<uint4 *>(static_cast<T *>(a.q) + (size_t)row * a.q_stride + (size_t)head * kDim + in), out);
-                } else if (there) {
-                    const uint32_t h = is_v ? head - a.q_heads - c.heads : head - a.q_heads;
-                    T *pool = reinterpret_cast<T *>(is_v ? c.v : c.k);
-                    const size_t slab = ((size_t)a.layer * c.pages + at.page) * c.heads + h;
-                    *reinterpret_cast<uint4 *>(pool + ((slab << c.page_shift) + (size_t)(at.pos & (c.page - 1))) * kDim + in) = out;
-                }
+                if (is_q) __stcs(reinterpret_cast<uint4 *>(q_row + (size_t)head * kDim), out);
+                else if (there) *reinterpret_cast<uint4 *>((is_v ? v_row + (size_t)(head - a.q_heads - c.heads) * head_step : k_row + (size_t)(head - a.q_heads) * head_step)) = out;
             }
 #pragma unroll
             for (int k = 0; k < kAhead; ++k) got[k] = next[k];
