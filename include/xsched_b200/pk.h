@@ -316,7 +316,8 @@ xpkResult xpkKvAppend(xpkKvCache_t cache, const xpkKvAppendArgs *args, void *str
  * `scratch`: xpkAttentionScratchBytes bytes, 256-byte aligned, zeroed once before its first use; a call leaves it ready
  * for the next one on the same cache, whatever its sizes.  Calls that may overlap on the GPU (other streams, other captured graphs)
  * need scratch of their own.
- * A call that was refused wrote nothing.  n <= XPK_ATTENTION_MAX_SEQS. */
+ * A call that was refused wrote nothing.  The call has no status channel: a bounded wait inside the kernel that gives up leaves
+ * `out` undefined (the task form reports it).  n <= XPK_ATTENTION_MAX_SEQS. */
 #define XPK_ATTENTION_MAX_SEQS 1024
 typedef struct {
     void *out;

@@ -556,6 +556,33 @@ def test_attention_task_stops_and_resumes_with_the_same_bytes(pk, kv):
     c.destroy()
 
 
+@pytest.mark.parametrize("counts", [[1, 1, 1, 1], [1, 30, 4, 1]])
+def test_a_flag_that_goes_up_and_down_while_the_kernel_runs(pk, kv, counts):
+    """A warp that saw the flag up has left tickets behind: it must not go on to a merge that waits for them once the flag is down."""
+    lens = [9000, 4000, 300, 12000]
+    c = _filled(pk, lens, 64, 4, 128, torch.bfloat16)
+    starts = np.concatenate([[0], np.cumsum(counts)]).tolist()
+    q = _normal(_gen(33), torch.bfloat16, starts[-1], 16, 128)
+    want = _attend(pk, c, q, None, _ints(starts), 4)
+    out = torch.zeros_like(q)
+    scratch = torch.zeros(c.attention_scratch_bytes(starts[-1], 4, 16), dtype=torch.uint8, device="cuda")
+    t = pk.Task.attention(c, out, q, None, scratch=scratch, starts=_ints(starts))
+    for _ in range(30):
+        out.zero_()
+        while True:
+            t.launch(_stream())
+            t.set_flag(1)
+            t.set_flag(0)
+            info = t.wait()
+            torch.cuda.synchronize()
+            assert info.status in (pk.STATUS_PREEMPTED, pk.STATUS_COMPLETED) and info.error == 0
+            if info.status == pk.STATUS_COMPLETED:
+                break
+        assert torch.equal(out, want)
+    t.destroy()
+    c.destroy()
+
+
 def test_two_streams_with_scratch_of_their_own(pk, kv):
     lens = [3000, 2500, 100]
     c = _filled(pk, lens, 16, 2, 64, torch.bfloat16)

@@ -28,38 +28,29 @@ namespace xpk {
 // finished, and a completed task's are cleared with the rest.
 constexpr int kTileTickets = 0, kUnitTickets = 1, kMergeTickets = 2;
 
+constexpr int kNone = -1, kStopped = -2;                     // every ticket is claimed; the flag was up (it may be down again)
+
 template <bool kPreemptible>
-__device__ __forceinline__ int claim(Ctl *ctl, const AttnShared *sh, int which, int total) {       // one thread; -1: none
-    if (*(const volatile uint32_t *)&sh->abort != 0u) return -1;
-    if constexpr (kPreemptible) { if (ld_flag(ctl->flag) != 0) return -1; }
+__device__ __forceinline__ int claim(Ctl *ctl, const AttnShared *sh, int which, int total) {       // one thread
+    if (*(const volatile uint32_t *)&sh->abort != 0u) return kStopped;
+    if constexpr (kPreemptible) { if (ld_flag(ctl->flag) != 0) return kStopped; }
     const unsigned long long t = atomicAdd(&ctl->user[which], 1ull);
-    return t < (unsigned long long)total ? (int)t : -1;
+    return t < (unsigned long long)total ? (int)t : kNone;
 }
 
-// A ticket for a warp.  Without tiles all warps come here at once, and where nothing can stop a launch its tickets begin at zero: the
-// first round is dealt by the warp's number (spread over the SMs), which saves the wait for a counter, 0.7 us; `dealt`: bit per counter.
+// A ticket for a warp.  Tickets are never dealt by the warp's number: a CTA that has not got an SM yet would hold some, and two launches
+// that share the SMs would wait for each other's.
 template <bool kPreemptible>
-__device__ __forceinline__ int warp_claim(Ctl *ctl, const AttnShared *sh, int which, int total, uint32_t &dealt) {
-    const bool deal = !kPreemptible && sh->tiles == 0;
-    const int warps = (int)gridDim.x * kWorkers;
-    if (deal && !(dealt >> which & 1u)) {
-        dealt |= 1u << which;
-        const int t = (int)(threadIdx.x >> 5) * (int)gridDim.x + (int)blockIdx.x;
-        return t < total && *(const volatile uint32_t *)&sh->abort == 0u ? t : -1;
-    }
-    if (deal && total <= warps) return -1;
-    int t = -1;
-    if ((threadIdx.x & 31) == 0) {
-        t = claim<kPreemptible>(ctl, sh, which, deal ? total - warps : total);
-        if (deal && t >= 0) t += warps;
-    }
+__device__ __forceinline__ int warp_claim(Ctl *ctl, const AttnShared *sh, int which, int total) {
+    int t = kNone;
+    if ((threadIdx.x & 31) == 0) t = claim<kPreemptible>(ctl, sh, which, total);
     return __shfl_sync(0xffffffffu, t, 0);
 }
 
 // An item from the loader; all lanes of a warp, or the issuing thread alone.
 __device__ __forceinline__ int next_item(AttnShared *sh, Ctl *ctl, uint32_t &seen) {
     const uint32_t slot = seen % kSched;
-    if (!wait_bar(&sh->item_full[slot], (seen / kSched) & 1u, sh, ctl, kErrAttnTile)) return -1;
+    if (!wait_bar(&sh->item_full[slot], (seen / kSched) & 1u, sh, ctl, kErrAttnTile)) return kStopped;
     ++seen;
     return *(volatile int *)&sh->item[slot];
 }
@@ -73,11 +64,12 @@ __device__ __forceinline__ void workers(Ctl *ctl, const CUtensorMap *map_k, cons
     unsigned char *const unit_ring = smem + (size_t)warp * kUnitStages * unit_stage_bytes<kDim>();
     Ring ring{unit_ring, sh->full[warp], kUnitStages, 0u, 0u, 0u, 0u};
     unsigned long long done = 0;
-    uint32_t dealt = 0;
+    bool stopped = false;                                   // somewhere tickets may be left
     for (int phase = 0; phase < 2; ++phase) {
         if ((phase == 0) != tiles_first) {
             while (sh->units > 0) {
-                const int ticket = warp_claim<kPreemptible>(ctl, sh, kUnitTickets, sh->units, dealt);
+                const int ticket = warp_claim<kPreemptible>(ctl, sh, kUnitTickets, sh->units);
+                stopped = stopped || ticket == kStopped;
                 if (ticket < 0) break;
                 unit_ticket<T, kDim>(c, a, map_k, map_v, sh, ctl, ring, ticket);
                 done += lane == 0;
@@ -90,6 +82,7 @@ __device__ __forceinline__ void workers(Ctl *ctl, const CUtensorMap *map_k, cons
             while (true) {
                 const uint32_t slot = seen % kSched;
                 const int ticket = __shfl_sync(0xffffffffu, next_item(sh, ctl, seen), 0);
+                stopped = stopped || ticket == kStopped;
                 if (ticket < 0) break;
                 const TileItem x = tile_ticket(a, c, sh, ticket);
                 __syncwarp();
@@ -105,9 +98,10 @@ __device__ __forceinline__ void workers(Ctl *ctl, const CUtensorMap *map_k, cons
             ring.move(unit_ring, kUnitStages);
         }
     }
-    // Without anything to do there is one merge of nothing, so that the call has a ticket to complete.
-    while (true) {
-        const int ticket = warp_claim<kPreemptible>(ctl, sh, kMergeTickets, sh->merges, dealt);
+    // Merges wait for every unit and tile: only once all of them are claimed, by warps that finish them, may one be begun.  Without
+    // anything to do there is one merge of nothing, so that the call has a ticket to complete.
+    while (!stopped) {
+        const int ticket = warp_claim<kPreemptible>(ctl, sh, kMergeTickets, sh->merges);
         if (ticket < 0) break;
         run_merge<T, kDim>(c, a, sh, ctl, ticket);
         done += lane == 0;
@@ -131,7 +125,7 @@ __device__ __forceinline__ void helpers(Ctl *ctl, const CUtensorMap *page_k, con
         const int lane = threadIdx.x & 31;
         uint32_t stage = 0, given = 0, keys0 = 0, keys1 = 0, ends = 0;
         while (true) {
-            int ticket = -1;
+            int ticket = kNone;
             if (lane == 0) ticket = claim<kPreemptible>(ctl, sh, kTileTickets, sh->tiles);
             ticket = __shfl_sync(0xffffffffu, ticket, 0);
             const uint32_t slot = given % kSched;

@@ -10,21 +10,28 @@ constexpr int kWorkers = 8;                                 // warps that run un
 constexpr int kUnitThreads = kWorkers * 32;
 constexpr int kAttnThreads = kUnitThreads + 128;            // and a third group for tiles: one warp loads, one issues MMAs
 // Registers: 384 threads are launched with 168 each; the workers, whose rows of scores fill 128, take over what the helpers
-// do not need: 2 * 208 + 88 = 3 * 168.
-constexpr int kWorkerRegs = 208, kHelperRegs = 88;
+// do not need: 2 * 216 + 72 = 3 * 168.
+constexpr int kWorkerRegs = 216, kHelperRegs = 72;
 static_assert(2 * kWorkerRegs + kHelperRegs <= 3 * 168, "more registers than the launch has");
 constexpr int kBlock = 16;                                  // positions per block of a unit
 constexpr int kUnitRows = 16;                               // rows of a unit, and of a partial result
-constexpr int kUnitRowsMost = 32;                           // sequences of more rows go by tiles
+// Sequences of up to 32 rows go by units (two groups read the same keys, the second from L2), longer ones by tiles: 40 drafts of up to 24
+// rows take 53 us, and 56 with the border at 16.
+constexpr int kUnitRowsMost = 32;
 constexpr int kUnitStages = 3;
-constexpr int kUnitWaves = 2;                               // units that each warp gets where there is enough work
+// Units that each warp gets where there is enough work: each begins by waiting for memory, so more and shorter ones are slower (32 sequences
+// apart: 112 us with two, 117 with three, 130 with five).
+constexpr int kUnitWaves = 2;
 constexpr int kTile = 128;                                  // positions per tile; rows per group of a tile item
 constexpr int kItemRows = 2 * kTile;
 constexpr int kStep = 64;                                   // positions per product; tiles are counted in pairs of steps
 constexpr int kRing = 8;                                    // stages of the tile ring; a stage holds a step's keys or values
 constexpr int kMinRun = 4;                                  // blocks: a run shorter than 64 positions costs more to merge than it spreads
-constexpr int kMinTiles = 4;                                // tiles: two for each group of workers
-constexpr int kShareRows = 64;                              // sequences of more rows fill tiles by themselves
+// Tiles of a run at least, two for each group of workers: 16 sequences on 4096 take 35 us, and 39 with runs of 2 (twice the results to merge).
+constexpr int kMinTiles = 4;
+// Sequences of more rows read the prefix by themselves: they fill half a group's tile.  12 sequences of 48 rows on a prefix of 8192 take
+// 78 us together and 140 each for itself.
+constexpr int kShareRows = 64;
 constexpr int kMergeRowsMost = 32;
 constexpr int kPageWords = 16;                              // more than the steps that a ring holds
 constexpr int kSched = 2;                                   // items the loader may be ahead
