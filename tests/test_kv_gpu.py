@@ -406,6 +406,25 @@ def test_as_many_sequences_as_a_call_takes(pk, kv, shared):
     c.destroy()
 
 
+def test_a_prefix_whose_results_do_not_fit_the_scratch_is_read_by_each_sequence(pk, kv):
+    """720 x 64 key heads x 2 row groups leave more results than the scratch takes: the call goes without the prefix."""
+    n, H, G, D, t = 720, 64, 8, 64, 3
+    lens = [66 + i % 5 for i in range(n)]
+    c = _filled(pk, lens, 64, H, D, torch.bfloat16)
+    _share(c, lens, 64)
+    starts = [t * i for i in range(n + 1)]
+    q = _normal(_gen(34), torch.bfloat16, starts[-1], H * G, D)
+    out = _attend(pk, c, q, None, _ints(starts), n, shared=64)
+    some = [0, 1, 17, 359, 700, 719]
+    rows = [starts[i] + j for i in some for j in range(t)]
+    table = c.page_table[some].contiguous()
+    small = pk.KvCache(c.k, c.v, table, _ints([lens[i] for i in some]), c.refs)
+    _check(kv, small, q[rows], out[rows], list(range(len(some))), [t * i for i in range(len(some) + 1)])
+    assert bool(torch.isfinite(out).all()) and not bool((out == 7).any())
+    c.destroy()
+    small.destroy()
+
+
 def test_missing_pages_are_left_out(pk, kv):
     lens = [300, 64, 20]
     c = _filled(pk, lens, 16, 2, 128, torch.float16)

@@ -20,7 +20,7 @@ constexpr int kUnitRows = 16;                               // rows of a unit, a
 constexpr int kUnitRowsMost = 32;
 constexpr int kUnitStages = 3;
 // Units that each warp gets where there is enough work: each begins by waiting for memory, so more and shorter ones are slower (32 sequences
-// apart: 112 us with two, 117 with three, 130 with five).
+// apart: 112 us with two, 117 with three, 130 with five, before runs were made equally long).
 constexpr int kUnitWaves = 2;
 constexpr int kTile = 128;                                  // positions per tile; rows per group of a tile item
 constexpr int kItemRows = 2 * kTile;
