@@ -1,0 +1,76 @@
+"""Attention over the paged cache at the borders of its cut: how many results a call leaves, where they go, and what the
+tiles do that ordinary scores hardly reach.  Tolerances are those of test_kv_gpu.py."""
+import random
+
+import numpy as np
+import pytest
+
+pytestmark = pytest.mark.gpu
+
+torch = pytest.importorskip("torch")
+
+from oracle import attention_cut as ac                                       # noqa: E402
+from test_kv_gpu import TYPES, _attend, _check, _filled, _gen, _ints, _normal, _share, _stream, kv, pk      # noqa: E402,F401
+
+
+def _sms():
+    return torch.cuda.get_device_properties(0).multi_processor_count
+
+
+def _starts(counts):
+    return np.concatenate([[0], np.cumsum(counts)]).tolist()
+
+
+def _check_some(pk, kv, c, q, out, counts, lens, some, scale=None):
+    """The rows of a few of the sequences against the definition."""
+    starts = _starts(counts)
+    rows = [starts[i] + j for i in some for j in range(counts[i])]
+    small = pk.KvCache(c.k, c.v, c.page_table[some].contiguous(), _ints([lens[i] for i in some]), c.refs)
+    _check(kv, small, q[rows], out[rows], list(range(len(some))), _starts([counts[i] for i in some]), scale=scale)
+    small.destroy()
+
+
+@pytest.mark.parametrize("n, t, q_heads, heads, length", [(200, 128, 32, 32, 500), (512, 16, 128, 16, 100), (1024, 32, 32, 8, 40)])
+def test_many_short_prompts_stay_inside_their_scratch(pk, kv, n, t, q_heads, heads, length):
+    """33 to 128 rows a sequence, more of them than two results a row group have room for; a guard behind the scratch stays as it was."""
+    c = _filled(pk, [length] * n, 64, heads, 64, torch.float16)
+    q = _normal(_gen(40), torch.float16, n * t, q_heads, 64)
+    bytes_ = c.attention_scratch_bytes(n * t, n, q_heads)
+    guard = (1 << 16) * ac.UNIT_ROWS * 64 * 4
+    buffer = torch.zeros(bytes_ + guard, dtype=torch.uint8, device="cuda")
+    buffer[bytes_:] = 0x5A
+    out = _attend(pk, c, q, None, _ints(_starts([t] * n)), n, scratch=buffer[:bytes_])
+    assert bool((buffer[bytes_:] == 0x5A).all())
+    assert bool(torch.isfinite(out).all()) and not bool((out == 7).all(-1).any())
+    _check_some(pk, kv, c, q, out, [t] * n, [length] * n, [0, n // 2, n - 1])
+    c.destroy()
+
+
+def test_tickets_and_scratch_are_those_of_the_cpu_cut(pk, kv):
+    """What the kernel counts as a task's tiles, and the scratch that the library asks for, over random calls."""
+    rng = random.Random(3)
+    for i in range(24):
+        heads, group, dim, page = rng.choice([1, 2, 8]), rng.choice([1, 4, 8]), rng.choice([64, 128]), rng.choice([16, 64])
+        n = rng.choice([1, 3, 40, 200])
+        counts = [1] * n if i % 3 == 0 else [rng.choice([1, 1, 3, rng.randint(1, 40)]) for _ in range(n)]
+        shared = rng.choice([0, 192, 1024])
+        lens = [rng.choice([-1, 0, shared + rng.randint(40, 900), shared + rng.randint(40, 900)]) for _ in range(n)]
+        c = _filled(pk, [max(x, 0) for x in lens], page, heads, dim, torch.bfloat16)
+        first = next((k for k in range(n) if lens[k] >= shared), 0)
+        for k in range(n):
+            if shared and lens[k] >= shared:
+                c.page_table[k, :shared // page] = c.page_table[first, :shared // page]
+        rows, q_heads = sum(counts), heads * group
+        assert c.attention_scratch_bytes(rows, n, q_heads) == ac.scratch_bytes(_sms(), heads, dim, rows, n, q_heads)
+        q = _normal(_gen(i), torch.bfloat16, rows, q_heads, dim)
+        out = torch.zeros_like(q)
+        scratch = torch.zeros(c.attention_scratch_bytes(rows, n, q_heads), dtype=torch.uint8, device="cuda")
+        seqs = _ints([-1 if x < 0 else k for k, x in enumerate(lens)])
+        t = pk.Task.attention(c, out, q, seqs, scratch=scratch, starts=_ints(_starts(counts)), shared_len=_ints([shared]) if shared else None)
+        t.launch(_stream())
+        info = t.wait()
+        x = ac.cut(_sms(), heads, dim, q_heads, page, counts, lens, shared, rows=rows)
+        assert info.status == pk.STATUS_COMPLETED and info.tiles_total == info.tiles_done == x.tiles + x.units + x.merges
+        torch.cuda.synchronize()
+        t.destroy()
+        c.destroy()

@@ -182,6 +182,7 @@ __device__ __forceinline__ void work_off(Ctl *ctl, const CUtensorMap *map_k, con
     if (threadIdx.x == 0) {
         // Never zero: a task that was stopped before any CTA got here must not look complete.
         *(volatile unsigned long long *)&ctl->total = (unsigned long long)sh->tiles + sh->units + merges;       // the same from every CTA
+        if (sh->abort != 0u) raise_error(ctl, kErrAttnCut);
     }
     if (tiles && warp == kWorkers + 1) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" :: "r"(smem_u32(&sh->tmem)), "r"(kAttnTmemCols) : "memory");
@@ -291,7 +292,8 @@ AttnScratch attention_scratch(const CacheView &c, uint32_t sms, uint32_t rows, u
     auto up = [](size_t x) { return (x + 255) & ~(size_t)255; };
     // Sequences of several runs leave less than twice work / run results, and a run is at least work / target (for tiles: 16
     // slots a result, two halves).  With a prefix every sharing sequence leaves some: one per key head if it is of one row
-    // group (all are where each has a single query of up to 16 heads), at most eight; the prefix itself 16 per item.
+    // group (all are where each has a single query of up to 16 heads), at most eight; the prefix itself 16 per item.  Sequences
+    // of 33 to 128 rows leave two per row group even in one run; the kernel cuts them without halves if they do not suffice.
     const size_t group = q_heads / c.heads, most = std::min<size_t>(n, rows);
     const size_t base = 2 * (size_t)kUnitWaves * sms * kWorkers + 128 * (size_t)sms;
     const size_t own = c.heads * most * (rows <= n && group <= kUnitRows ? 1 : 8);

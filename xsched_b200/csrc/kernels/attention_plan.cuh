@@ -39,6 +39,7 @@ constexpr float kTileUs = 2.6f;                             // measured time of 
 constexpr uint32_t kErrAttnLoad  = 0x70000001u;
 constexpr uint32_t kErrAttnMerge = 0x70000002u;
 constexpr uint32_t kErrAttnTile  = 0x70000003u;
+constexpr uint32_t kErrAttnCut   = 0x70000004u;
 
 struct AttnArgs {
     const void *q;
@@ -78,6 +79,7 @@ struct AttnShared {
     unsigned long long full[kWorkers][kUnitStages];
     unsigned long long done;
     int run, tile_run;                                      // blocks (tiles) per run
+    int half_rows;                                          // up to so many rows the two groups of workers take half of a run each
     int units, tiles, merges, merge_rows;
     int shared, shared_seq, pre_rows, pre_part0, pre_tiles; // prefix: positions, whose table, rows, first result, its tile items
     int tile_ctas;                                          // CTAs that begin with tiles
@@ -161,8 +163,9 @@ __device__ __forceinline__ long long rows_of(const SeqPlan &p, uint32_t group) {
 __device__ __forceinline__ bool by_tiles(const SeqPlan &p, uint32_t group) { return rows_of(p, group) > kUnitRowsMost; }
 __device__ __forceinline__ int row_groups(long long rows) { return (int)((rows + kUnitRows - 1) / kUnitRows); }
 __device__ __forceinline__ int row_tiles(long long rows) { return (int)((rows + kItemRows - 1) / kItemRows); }
-// With at most 128 rows the two groups of workers take half of a run's tiles each, and leave a result each.
-__device__ __forceinline__ int halves(long long rows) { return rows <= kTile ? 2 : 1; }
+// With at most 128 rows the two groups of workers take half of a run's tiles each, and leave a result each; where so many results
+// do not fit the scratch (half_rows 0) the first group takes all of them.
+__device__ __forceinline__ int halves(const AttnShared *sh, long long rows) { return rows <= sh->half_rows ? 2 : 1; }
 __device__ __forceinline__ int chunks(int positions, int each, int run) { return max(1, ((positions + each - 1) / each + run - 1) / run); }
 __device__ __forceinline__ int tiles_of(int positions) { return (positions + kTile - 1) / kTile; }
 // Runs of about tile_run tiles, equally long: the last item to end should not be a short one's neighbour.
@@ -173,9 +176,9 @@ __device__ __forceinline__ int tile_runs(const AttnShared *sh, int positions) {
 __device__ __forceinline__ int runs_of(const AttnShared *sh, uint32_t group, int i) {
     const SeqPlan &p = sh->plan[i];
     const int own = p.len - own_from(sh, i);
-    return by_tiles(p, group) ? tile_runs(sh, own) * halves(rows_of(p, group)) : chunks(own, kBlock, sh->run);
+    return by_tiles(p, group) ? tile_runs(sh, own) * halves(sh, rows_of(p, group)) : chunks(own, kBlock, sh->run);
 }
-__device__ __forceinline__ int pre_runs(const AttnShared *sh) { return tile_runs(sh, sh->shared) * halves(sh->pre_rows); }
+__device__ __forceinline__ int pre_runs(const AttnShared *sh) { return tile_runs(sh, sh->shared) * halves(sh, sh->pre_rows); }
 
 // ---- the cut ----------------------------------------------------------------------------------------------------
 __device__ __forceinline__ unsigned long long warp_sum(unsigned long long v) {
@@ -216,11 +219,14 @@ __device__ __forceinline__ void make_plan(const CacheView &c, const AttnArgs &a,
     }
     __syncthreads();
     if (sh->sums[3] < 2) shared = 0;
-    // A second round without the prefix if its results do not fit the scratch.
-    for (int round = 0; round < 2; ++round) {
+    // Results that do not fit the scratch: once more without the prefix, then without halves too.  What is left then is under
+    // 64 results per SM, by sequences of several runs alone; the scratch has room for 160.
+    bool halved = true;
+    while (true) {
         if (shared == 0 && tid < XPK_ATTENTION_MAX_SEQS / 32) sh->share[tid] = 0;
         if (tid == 0) {
             sh->shared = shared;
+            sh->half_rows = halved ? kTile : 0;
             sh->shared_seq = shared > 0 ? sh->plan[sh->first_sharing].seq : -1;
         }
         __syncthreads();
@@ -280,9 +286,9 @@ __device__ __forceinline__ void make_plan(const CacheView &c, const AttnArgs &a,
                 const SeqPlan p = sh->plan[i];
                 const long long rs = rows_of(p, a.group);
                 const int runs = runs_of(sh, a.group, (int)i), groups = row_groups(rs) * (int)c.heads;
-                if (by_tiles(p, a.group)) v.y = row_tiles(rs) * (int)c.heads * (runs / halves(rs));
+                if (by_tiles(p, a.group)) v.y = row_tiles(rs) * (int)c.heads * (runs / halves(sh, rs));
                 else v.x = groups * runs;
-                if (runs > 1 || shares(sh, (int)i)) v.z = groups * runs;
+                if (runs > 1 || shares(sh, (int)i)) v.z = (int)min((long long)groups * runs, (long long)a.part_slots + 1);      // the sum cannot wrap
                 if (shares(sh, (int)i)) v.w = (int)rs;
             }
             int4 s = v;
@@ -312,12 +318,17 @@ __device__ __forceinline__ void make_plan(const CacheView &c, const AttnArgs &a,
         }
         int parts = carry.z;
         if (shared > 0) parts += row_groups(sh->pre_rows) * (int)c.heads * pre_runs(sh);
-        if (shared > 0 && parts > (int)a.part_slots) {                        // the same for all threads
+        const bool fits = parts <= (int)a.part_slots;                         // the same for all threads
+        if (!fits && (shared > 0 || halved)) {
+            halved = halved && shared > 0;
             shared = 0;
             if (tid < 3 || tid == 4) sh->sums[tid] = 0;
             continue;
         }
+        // By the bound above the results fit now; if they ever did not, nothing is stored and a task reports it.
+        if (!fits) carry.x = carry.y = parts = 0;
         if (tid == 0) {
+            if (!fits) sh->abort = 1;
             sh->units = carry.x;
             sh->tiles = carry.y;
             sh->pre_tiles = pre_items;

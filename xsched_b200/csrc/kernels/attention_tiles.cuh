@@ -174,7 +174,7 @@ __device__ __forceinline__ TileItem tile_ticket(const AttnArgs &a, const CacheVi
         local = ticket - sh->tile0[lo];
     }
     const int runs = tile_runs(sh, own), tiles = row_tiles(all), run = local % runs;
-    x.half = halves(all);
+    x.half = halves(sh, all);
     // Late rows see most: they come first.
     const int rt = tiles - 1 - (local / runs) % tiles;
     x.head = local / (runs * tiles);
