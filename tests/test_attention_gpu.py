@@ -74,3 +74,32 @@ def test_tickets_and_scratch_are_those_of_the_cpu_cut(pk, kv):
         torch.cuda.synchronize()
         t.destroy()
         c.destroy()
+
+
+def test_a_prefix_that_just_does_not_fit_is_dropped_by_every_thread_alike(pk, kv):
+    """Results fit with the prefix's runs counted as one and do not with the real number: a thread that looked at the next round's
+    prefix would go on with another cut than the rest."""
+    m, s, heads, prefix = 696, 10, 8, 65536
+    counts, lens = [1] * s + [128] * m, [prefix + 40 + i for i in range(s)] + [128] * m
+    slots = ac.part_slots(_sms(), heads, sum(counts), s + m, heads)
+    share = np.arange(s + m) < s
+    _, _, parts = ac._round(_sms(), heads, 64, 1, np.array(counts), np.array(lens), prefix, share, True)
+    runs_as_one = 16 * heads * m + heads * s + 2 * heads
+    assert _sms() != 148 or runs_as_one <= slots < parts
+    c = _filled(pk, [lens[i] if i < s else 128 for i in range(s + m)], 128, heads, 64, torch.bfloat16)
+    _share(c, lens[:s], prefix)
+    q = _normal(_gen(41), torch.bfloat16, sum(counts), heads, 64)
+    starts = _ints(_starts(counts))
+    scratch = torch.zeros(c.attention_scratch_bytes(sum(counts), s + m, heads), dtype=torch.uint8, device="cuda")
+    out = _attend(pk, c, q, None, starts, s + m, shared=prefix, scratch=scratch)
+    _check_some(pk, kv, c, q, out, counts, lens, [0, s - 1, s, s + m - 1])
+    for _ in range(20):
+        assert torch.equal(_attend(pk, c, q, None, starts, s + m, shared=prefix, scratch=scratch), out)
+    t = pk.Task.attention(c, torch.zeros_like(q), q, None, scratch=scratch, starts=starts, shared_len=_ints([prefix]))
+    t.launch(_stream())
+    info = t.wait()
+    x = ac.cut(_sms(), heads, 64, heads, 128, counts, lens, prefix)
+    assert info.status == pk.STATUS_COMPLETED and info.tiles_total == x.tiles + x.units + x.merges
+    assert torch.equal(out, _attend(pk, c, q, None, starts, s + m, shared=prefix))
+    t.destroy()
+    c.destroy()

@@ -320,6 +320,7 @@ __device__ __forceinline__ void make_plan(const CacheView &c, const AttnArgs &a,
         if (shared > 0) parts += row_groups(sh->pre_rows) * (int)c.heads * pre_runs(sh);
         const bool fits = parts <= (int)a.part_slots;                         // the same for all threads
         if (!fits && (shared > 0 || halved)) {
+            __syncthreads();                                                  // the sum reads what the next round writes first
             halved = halved && shared > 0;
             shared = 0;
             if (tid < 3 || tid == 4) sh->sums[tid] = 0;
