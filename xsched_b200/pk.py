@@ -276,6 +276,8 @@ def _rows(what: str, x, width: int):
         if size != 1 and stride != inner:
             raise ValueError(f"{what}: a row's elements lie apart (strides {x.stride()})")
         inner *= size
+    if rows > 1 and x.stride(0) < width:                  # an expanded tensor has a step of 0, which would mean dense
+        raise ValueError(f"{what}: rows overlap (strides {x.stride()})")
     return rows, x.stride(0) if rows > 1 else 0
 
 
