@@ -1,0 +1,24 @@
+"""Pages of the key/value cache at sizes where sums and offsets could pass 32 bits, and under streams of their own."""
+import pytest
+
+pytestmark = pytest.mark.gpu
+
+torch = pytest.importorskip("torch")
+
+from test_kv_gpu import _ints, _stream, kv, pk      # noqa: E402,F401
+
+
+def test_extend_by_more_pages_than_a_32_bit_sum_holds_changes_nothing(pk, kv):
+    """512 sequences want 2^22 pages each: 2^31 in all, of which there are 40."""
+    n, width, page, pages = 512, 1 << 22, 16, 40
+    k = torch.zeros(1, pages, 1, page, 64, dtype=torch.bfloat16, device="cuda")
+    table = torch.empty(n, width, dtype=torch.int32, device="cuda")          # 8.6 GB, which nobody reads: all sequences are empty
+    c = pk.KvCache(k, torch.zeros_like(k), table, _ints([0] * n), _ints([0] * pages))
+    for each in (width, width // 2 + 1, width - 1):
+        c.extend(_ints(list(range(n))), _ints([each * page] * n), _stream())
+        r = c.result(_stream())
+        assert (r.copied, r.missing, r.refused) == (0, 1, 0)                 # as many as are counted: one more than there are
+        assert not bool(c.lens.any()) and not bool(c.refs.any())
+    c.extend(_ints([3, 7]), _ints([20 * page, 20 * page]), _stream())        # and what fits is given
+    assert c.result(_stream()).missing == 0 and c.lens[7].item() == 20 * page and bool((c.refs == 1).all())
+    c.destroy()

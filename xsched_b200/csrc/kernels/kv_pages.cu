@@ -85,27 +85,26 @@ __global__ void __launch_bounds__(256) kv_fork_kernel(CacheView c, KvWork w, con
 
 // ------------------------------------------------------------------------------------------------ scans of one CTA
 // Exclusive sum over the CTA's threads; `total` gets the sum of all.
-__device__ __forceinline__ int block_scan(int v, int *s_warp, int &total) {
+template <class N>
+__device__ __forceinline__ N block_scan(N v, N *s_warp, N &total) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    int x = v;
+    N x = v;
 #pragma unroll
     for (int d = 1; d < 32; d <<= 1) {
-        const int y = __shfl_up_sync(0xffffffffu, x, d);
+        const N y = __shfl_up_sync(0xffffffffu, x, d);
         if (lane >= d) x += y;
     }
     __syncthreads();                                        // s_warp of the call before has been read
     if (lane == 31) s_warp[warp] = x;
     __syncthreads();
-    int before = 0;
-    total = 0;
-    const int sum = lane < (int)(blockDim.x >> 5) ? s_warp[lane] : 0;
-    int y = sum;
+    const N sum = lane < (int)(blockDim.x >> 5) ? s_warp[lane] : 0;
+    N y = sum;
 #pragma unroll
     for (int d = 1; d < 32; d <<= 1) {
-        const int z = __shfl_up_sync(0xffffffffu, y, d);
+        const N z = __shfl_up_sync(0xffffffffu, y, d);
         if (lane >= d) y += z;
     }
-    before = __shfl_sync(0xffffffffu, y - sum, warp);
+    const N before = __shfl_sync(0xffffffffu, y - sum, warp);
     total = __shfl_sync(0xffffffffu, y, 31);
     return before + x - v;
 }
@@ -116,6 +115,7 @@ __global__ void __launch_bounds__(kPlanThreads) kv_extend_kernel(CacheView c, Kv
     constexpr int kEach = XPK_KV_MAX_LIST / kPlanThreads;
     __shared__ int s_seq[XPK_KV_MAX_LIST], s_tail[XPK_KV_MAX_LIST], s_off[XPK_KV_MAX_LIST];
     __shared__ int s_warp[32], s_copied;
+    __shared__ long long s_warp_need[32];
     const int tid = threadIdx.x;
     int held[kEach], grow[kEach];
     bool again[kEach];
@@ -176,11 +176,12 @@ __global__ void __launch_bounds__(kPlanThreads) kv_extend_kernel(CacheView c, Kv
                 else need = (int)has - pages_of(c, held[e]) + (split[e] ? 1 : 0);
             }
         }
-        int total;
-        const int before = block_scan(need, s_warp, total);
-        if (i < (int)n) s_off[i] = carry + before;
-        // More than every page there is stays more; the sum cannot wrap.
-        carry = (int)min((long long)carry + total, (long long)c.pages + 1);
+        // In 64 bits: an entry may want as many pages as a table row has, 2^26, and 1024 of them are summed.  More than every page
+        // there is stays more; offsets count only if no page is missing.
+        long long total;
+        const long long before = block_scan((long long)need, s_warp_need, total), most = (long long)c.pages + 1;
+        if (i < (int)n) s_off[i] = (int)min(carry + before, most);
+        carry = (int)min(carry + total, most);
     }
     int all_refused;
     block_scan(refused, s_warp, all_refused);
