@@ -332,7 +332,8 @@ typedef struct {
 } xpkAttentionArgs;
 size_t    xpkAttentionScratchBytes(xpkKvCache_t cache, uint32_t rows, uint32_t n, uint32_t q_heads);
 xpkResult xpkAttention(xpkKvCache_t cache, const xpkAttentionArgs *args, void *stream);
-/* The same as a preemptible task.  Its scratch is its own, and is cleared here.  Lengths and tables are not to change between a
+/* The same as a preemptible task.  Its scratch is its own; what has to be zero in it is cleared here and, unless that launch is
+ * captured, by the first launch on its stream.  Lengths and tables are not to change between a
  * launch that was preempted and the one that finishes it. */
 xpkResult xpkTaskCreateAttention(xpkTask_t *task, xpkKvCache_t cache, const xpkAttentionArgs *args, uint32_t flags,
                                  uint32_t *flag_dev);

@@ -103,3 +103,44 @@ def test_a_prefix_that_just_does_not_fit_is_dropped_by_every_thread_alike(pk, kv
     assert torch.equal(out, _attend(pk, c, q, None, starts, s + m, shared=prefix))
     t.destroy()
     c.destroy()
+
+
+def test_a_task_created_while_its_scratch_is_still_written_on_another_stream(pk, kv):
+    """The scratch's last writer is queued on the stream that the task will run on, behind the creation's own clearing."""
+    lens = [9000, 4000, 300, 12000]
+    c = _filled(pk, lens, 64, 4, 128, torch.bfloat16)
+    q = _normal(_gen(42), torch.bfloat16, 4, 16, 128)
+    want = _attend(pk, c, q, None, None, 4)
+    s = torch.cuda.Stream()
+    scratch, out = torch.empty(c.attention_scratch_bytes(4, 4, 16), dtype=torch.uint8, device="cuda"), torch.zeros_like(q)
+    torch.cuda.synchronize()
+    with torch.cuda.stream(s):
+        torch.cuda._sleep(100_000_000)
+        scratch.fill_(0x7F)
+    t = pk.Task.attention(c, out, q, None, scratch=scratch)
+    for _ in range(2):
+        t.launch(s.cuda_stream)
+        assert t.wait().status == pk.STATUS_COMPLETED
+        torch.cuda.synchronize()
+        assert torch.equal(out, want)
+        out.zero_()
+        torch.cuda.synchronize()
+    t.destroy()
+    # The first launch captured: nothing is cleared in the graph, and its replays and a direct launch all work.
+    t = pk.Task.attention(c, out, q, None, scratch=scratch)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        t.launch(_stream())
+    for _ in range(2):
+        out.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want)
+    out.zero_()
+    t.launch(_stream())
+    assert t.wait().status == pk.STATUS_COMPLETED
+    torch.cuda.synchronize()
+    assert torch.equal(out, want)
+    del graph
+    t.destroy()
+    c.destroy()

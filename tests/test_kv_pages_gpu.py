@@ -22,3 +22,24 @@ def test_extend_by_more_pages_than_a_32_bit_sum_holds_changes_nothing(pk, kv):
     c.extend(_ints([3, 7]), _ints([20 * page, 20 * page]), _stream())        # and what fits is given
     assert c.result(_stream()).missing == 0 and c.lens[7].item() == 20 * page and bool((c.refs == 1).all())
     c.destroy()
+
+
+def test_a_cache_is_ready_for_streams_that_do_not_wait_for_the_default_one(pk, kv):
+    """The handle's workspace is cleared when the constructor returns, whatever the default stream is still doing."""
+    k = torch.zeros(1, 8, 1, 16, 64, dtype=torch.bfloat16, device="cuda")
+    v, refs, lens = torch.zeros_like(k), _ints([1] + [0] * 7), _ints([5, 0, 0])
+    table = _ints([[0, -1], [-1, -1], [-1, -1]])
+    parents, children = _ints([0, 0]), _ints([1, 2])
+    s = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    for _ in range(3):
+        torch.cuda._sleep(1_000_000_000)
+        c = pk.KvCache(k, v, table, lens, refs)
+        c.fork(parents, children, s.cuda_stream)
+        s.synchronize()
+        with torch.cuda.stream(s):
+            assert lens.tolist() == [5, 5, 5] and refs[0].item() == 3
+        c.free(children, s.cuda_stream)
+        s.synchronize()
+        torch.cuda.synchronize()
+        c.destroy()

@@ -60,6 +60,14 @@ xpkResult done(cudaError_t e, unsigned launches) {
     return XPK_SUCCESS;
 }
 
+// Clears new memory and waits for that alone: streams that do not wait for the default stream may use it once this returns.
+bool cleared(void *at, size_t bytes) {
+    cudaStream_t st;
+    if (cudaStreamCreateWithFlags(&st, cudaStreamNonBlocking) != cudaSuccess) return false;
+    const bool ok = cudaMemsetAsync(at, 0, bytes, st) == cudaSuccess && cudaStreamSynchronize(st) == cudaSuccess;
+    return cudaStreamDestroy(st) == cudaSuccess && ok;
+}
+
 void free_cache(xpkKvCache_st *c) {
     if (c->work) cudaFree(c->work);
     delete c;
@@ -121,7 +129,7 @@ xpkResult xpkKvCacheCreate(xpkKvCache_t *cache, const xpkKvCacheDesc *desc) {
     c->sms = xpk::device_sms();
     if (c->sms == 0 || cudaGetDevice(&c->device) != cudaSuccess) { free_cache(c); return XPK_ERR_CUDA; }
     const size_t bytes = xpk::kv_work_bytes(d.pages);
-    if (cudaMalloc((void **)&c->work, bytes) != cudaSuccess || cudaMemset(c->work, 0, bytes) != cudaSuccess) { free_cache(c); return XPK_ERR_CUDA; }
+    if (cudaMalloc((void **)&c->work, bytes) != cudaSuccess || !cleared(c->work, bytes)) { free_cache(c); return XPK_ERR_CUDA; }
     if (!pool_map(c->map_k, d, d.k, 16) || !pool_map(c->map_v, d, d.v, 16) ||
         !pool_map(c->page_k, d, d.k, std::min(d.page_size, 64u)) || !pool_map(c->page_v, d, d.v, std::min(d.page_size, 64u))) { free_cache(c); return XPK_ERR_CUDA; }
     const xpkResult r = attention_ready(c->device);
@@ -241,7 +249,9 @@ xpkResult xpkTaskCreateAttention(xpkTask_t *task, xpkKvCache_t cache, const xpkA
         t->cache = cache;
         t->attention = x;
         xpk::attention_counters(view_of(cache), cache->sms, x, &t->clear_at, &t->clear_bytes);
-        if (cudaMemset(t->clear_at, 0, t->clear_bytes) != cudaSuccess) r = XPK_ERR_CUDA;
+        // Once here, waited for, and once by the first launch on its own stream: what used the memory before may be queued there still.
+        if (cudaMemset(t->clear_at, 0, t->clear_bytes) != cudaSuccess || cudaStreamSynchronize(cudaStreamLegacy) != cudaSuccess) r = XPK_ERR_CUDA;
+        t->clear_first = true;
     }
     if (r != XPK_SUCCESS) { xpk::task_free(t); return r; }
     *task = t;

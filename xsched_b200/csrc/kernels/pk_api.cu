@@ -367,7 +367,14 @@ xpkResult xpkTaskLaunch(xpkTask_t t, void *stream, int sm_limit) {
                              t->M, t->N, t->K, launch_no, (int)grid, s);
         break;
     case XPK_KIND_ATTENTION:
-        e = xpk::launch_attention(preemptible, t->ctl, t->cache, t->attention, launch_no, sms, s);
+        if (t->clear_first.exchange(false)) {
+            // A graph does without: its later replays would clear what a preempted one has left.
+            cudaStreamCaptureStatus capture = cudaStreamCaptureStatusNone;
+            e = cudaStreamIsCapturing(s, &capture);
+            if (e == cudaSuccess && capture == cudaStreamCaptureStatusNone) e = cudaMemsetAsync(t->clear_at, 0, t->clear_bytes, s);
+            if (e != cudaSuccess) t->clear_first.store(true);
+        }
+        if (e == cudaSuccess) e = xpk::launch_attention(preemptible, t->ctl, t->cache, t->attention, launch_no, sms, s);
         break;
     case XPK_KIND_KV_COPY:
         e = xpk::launch_kv_copy_task(preemptible, t->ctl, view_of(t->cache), (const int32_t *)t->p1, (const int32_t *)t->p2, (uint32_t)t->n,

@@ -37,6 +37,7 @@ struct xpkTask_st {
     xpkAttentionArgs attention = {};
     void *clear_at = nullptr;         // what a reset clears besides the control block
     size_t clear_bytes = 0;
+    std::atomic<bool> clear_first{false};  // and the first launch
 };
 
 namespace xpk {
