@@ -144,3 +144,78 @@ def test_a_task_created_while_its_scratch_is_still_written_on_another_stream(pk,
     del graph
     t.destroy()
     c.destroy()
+
+
+def _levels(c, i, n, levels):
+    """Keys of sequence i: position p points along one direction, 64 positions at a time as far as `levels` says, plus noise."""
+    page, dim = c.k.shape[3], c.dim
+    pos = torch.arange(n, device="cuda")
+    at = torch.tensor([levels[p % len(levels)] for p in range(-(-n // 64))], device="cuda").repeat_interleave(64)[:n]
+    where = c.page_table[i].long()[pos // page]
+    k = 0.05 * c.k[0][where, :, pos % page].float()
+    k[..., 0] += at[:, None]
+    c.k[0][where, :, pos % page] = k.to(c.dtype)
+
+
+# How far the maximum lies, in units of a score, from 64 positions to the next: up by little and by much, down, and up again from far below.
+RISING, FALLING, ZIGZAG = [0.0, 3.0, 9.0, 14.0, 14.5, 22.0, 40.0, 41.0], [30.0, 12.0, 3.0, 0.0], [5.0, 30.0, -20.0, 31.0, 60.0, -60.0, 58.0, 59.0, 75.0]
+
+
+@pytest.mark.parametrize("dtype, Hq, H, D, page", [("bf16", 8, 2, 128, 64), ("fp16", 6, 2, 64, 16), ("fp16", 3, 1, 128, 128)])
+@pytest.mark.parametrize("levels", [RISING, FALLING, ZIGZAG])
+@pytest.mark.parametrize("scale", [1.0, -1.0])
+@pytest.mark.parametrize("shared, counts, lens", [(0, [20, 300, 9], [700, 900, 64]), (640, [1, 2, 5, 2], [700, 641, 1500, 650])])
+def test_tiles_follow_a_maximum_that_moves(pk, kv, dtype, Hq, H, D, page, levels, scale, shared, counts, lens):
+    """Results are scaled down wherever a row's maximum grows by more than 2^8; a negative scale turns the queries over."""
+    c = _filled(pk, lens, page, H, D, TYPES[dtype])
+    if shared:
+        _share(c, lens, shared)
+    for i, n in enumerate(lens):
+        if not shared or i == 0:
+            _levels(c, i, n, levels)
+    starts = _starts(counts)
+    q = 0.3 * _normal(_gen(43), torch.float32, starts[-1], Hq, D)
+    q[..., 0] = scale
+    q = q.to(TYPES[dtype])
+    out = _attend(pk, c, q, None, _ints(starts), len(lens), shared=shared or None, scale=scale)
+    _check(kv, c, q, out, list(range(len(lens))), starts, scale=scale)
+    c.destroy()
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("shared", [None, 256])
+@pytest.mark.parametrize("scale", [0.0, 0.5, -0.125])
+def test_tiles_with_scores_of_hundreds_equal_scores_and_odd_scales(pk, kv, dtype, shared, scale):
+    lens, counts = [700, 300, 333], [1, 2, 3] if shared else [140, 9, 40]
+    c = _filled(pk, lens, 32, 1, 64, TYPES[dtype])
+    if shared:
+        _share(c, lens, shared)
+    starts = _starts(counts)
+    q = _normal(_gen(44), TYPES[dtype], starts[-1], 12, 64, scale=30.0)
+    _check(kv, c, q, _attend(pk, c, q, None, _ints(starts), 3, shared=shared, scale=scale), [0, 1, 2], starts, scale=scale)
+    q.zero_()
+    _check(kv, c, q, _attend(pk, c, q, None, _ints(starts), 3, shared=shared, scale=scale), [0, 1, 2], starts, scale=scale)
+    c.destroy()
+
+
+def test_calls_and_grids_of_any_size_write_the_same_bytes(pk, kv):
+    """Single tokens, drafts, a prompt and a shared prefix in one call: repeated, and as a task on 1, 7 and all SMs."""
+    lens, counts = [5000, 4200, 4800, 4100, 6000, 4097], [1, 1, 4, 2, 150, 1]
+    c = _filled(pk, lens, 64, 2, 128, torch.bfloat16)
+    _share(c, lens, 4096)
+    starts = _ints(_starts(counts))
+    q = _normal(_gen(45), torch.bfloat16, sum(counts), 8, 128, scale=2.0)
+    scratch = torch.zeros(c.attention_scratch_bytes(sum(counts), 6, 8), dtype=torch.uint8, device="cuda")
+    want = _attend(pk, c, q, None, starts, 6, shared=4096, scratch=scratch)
+    for _ in range(20):
+        assert torch.equal(_attend(pk, c, q, None, starts, 6, shared=4096, scratch=scratch), want)
+    out = torch.zeros_like(q)
+    t = pk.Task.attention(c, out, q, None, scratch=torch.zeros_like(scratch), starts=starts, shared_len=_ints([4096]))
+    for sms in (1, 7, 0):
+        out.zero_()
+        t.launch(_stream(), sm_limit=sms)
+        assert t.wait(10_000_000).status == pk.STATUS_COMPLETED
+        torch.cuda.synchronize()
+        assert torch.equal(out, want)
+    t.destroy()
+    c.destroy()
