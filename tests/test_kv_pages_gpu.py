@@ -43,3 +43,26 @@ def test_a_cache_is_ready_for_streams_that_do_not_wait_for_the_default_one(pk, k
         s.synchronize()
         torch.cuda.synchronize()
         c.destroy()
+
+
+def test_calls_refuse_tensors_that_require_a_gradient(pk, kv):
+    from test_kv_gpu import _filled
+    c = _filled(pk, [20, 30], 16, 2, 64, torch.bfloat16)
+    q = torch.ones(2, 4, 64, dtype=torch.bfloat16, device="cuda")
+    out, qkv, inv = torch.zeros_like(q), torch.ones(2, 8 * 64, dtype=torch.bfloat16, device="cuda"), torch.ones(32, dtype=torch.float64, device="cuda")
+    w = torch.ones(64, dtype=torch.bfloat16, device="cuda")
+    scratch = torch.zeros(c.attention_scratch_bytes(2, 2, 4), dtype=torch.uint8, device="cuda")
+    grad = lambda x: x.clone().requires_grad_()
+    calls = [lambda: c.attention(out, grad(q), None, _stream(), scratch=scratch), lambda: c.attention(grad(out), q, None, _stream(), scratch=scratch),
+             lambda: pk.Task.attention(c, out, grad(q), None, scratch=scratch), lambda: c.append(grad(q), qkv, None, _stream()),
+             lambda: c.append(q, grad(qkv), None, _stream()), lambda: c.append(q, qkv, None, _stream(), inv_freq=grad(inv)),
+             lambda: c.append(q, qkv, None, _stream(), q_weight=grad(w), k_weight=w), lambda: pk.KvCache(grad(c.k), c.v, c.page_table, c.lens, c.refs)]
+    for call in calls:
+        with pytest.raises(ValueError, match="no_grad"):
+            call()
+    with torch.no_grad():
+        c.append(q, grad(qkv), None, _stream(), inv_freq=inv, q_weight=grad(w), k_weight=w)
+        c.attention(out, grad(q), None, _stream(), scratch=scratch)
+    torch.cuda.synchronize()
+    assert bool(out.any())
+    c.destroy()

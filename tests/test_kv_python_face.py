@@ -15,3 +15,19 @@ def test_rows_that_overlap_are_refused():
     assert pk._rows("q", torch.zeros(3, 4, 8), 32) == (3, 0)
     with pytest.raises(ValueError, match="apart"):
         pk._rows("q", torch.zeros(3, 1, 8).expand(3, 4, 8), 32)
+
+
+def test_tensors_that_require_a_gradient_are_refused_under_grad_mode():
+    """No backward pass is recorded: without the refusal their gradients would silently be missing."""
+    x = torch.zeros(2, 8, requires_grad=True)
+    for y in (x, x * 2, (x * 2)[:1]):
+        with pytest.raises(ValueError, match="no_grad"):
+            pk._no_gradient("q", y)
+    with torch.no_grad():
+        pk._no_gradient("q", x)
+    pk._no_gradient("q", x.detach())
+    cache = pk.KvCache.__new__(pk.KvCache)
+    cache.dtype, cache.device = x.dtype, x.device
+    with pytest.raises(ValueError, match="qkv requires a gradient"):
+        cache._data("qkv", x)
+    assert cache._data("qkv", x.detach()) == x.data_ptr()

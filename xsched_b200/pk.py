@@ -263,6 +263,14 @@ class Task:
             self._keep = ()
 
 
+def _no_gradient(what: str, x) -> None:
+    """The cache's kernels have no backward pass: what autograd would follow through them is refused, not lost."""
+    if x.requires_grad:
+        import torch
+        if torch.is_grad_enabled():
+            raise ValueError(f"{what} requires a gradient, and this call has none to give: call it under torch.no_grad()")
+
+
 def _rows(what: str, x, width: int):
     """(rows, elements between rows) of a tensor whose trailing dimensions, `width` elements in all, are dense."""
     shape = x.shape
@@ -286,7 +294,9 @@ class KvCache:
 
     k, v [layers, pages, kv_heads, page_size, head_dim] (bf16 or fp16), page_table [seqs, width], lens [seqs] and refs [pages]
     (int32) are the caller's tensors on one device and stay where they are.  Calls take the stream they run on; lists and
-    lengths are read on the device when the kernels run.  destroy() gives the handle back."""
+    lengths are read on the device when the kernels run.  destroy() gives the handle back.
+
+    For inference: nothing is recorded for autograd, and tensors that require a gradient are refused unless under torch.no_grad()."""
 
     def __init__(self, k, v, page_table, lens, refs):
         dtype = {"torch.bfloat16": DTYPE_BF16, "torch.float16": DTYPE_F16}.get(str(k.dtype))
@@ -303,6 +313,7 @@ class KvCache:
         for name, x in (("k", k), ("v", v), ("page_table", page_table), ("lens", lens), ("refs", refs)):
             if not x.is_contiguous() or x.device != k.device or not x.is_cuda:
                 raise ValueError(f"{name} is contiguous and on the same CUDA device as k")
+            _no_gradient(name, x)
         self.k, self.v, self.page_table, self.lens, self.refs = k, v, page_table, lens, refs
         self.device, self.dtype, self.heads, self.dim, self.seqs = k.device, k.dtype, heads, dim, lens.numel()
         self._int32 = lens.dtype
@@ -338,6 +349,7 @@ class KvCache:
             return None
         if x.dtype is not self.dtype or x.device != self.device:
             raise ValueError(f"{what} is {self.dtype} on {self.device}, got {x.dtype} on {x.device}")
+        _no_gradient(what, x)
         return x.data_ptr()
 
     def _entries(self, seqs, starts, rows: int) -> int:
@@ -390,6 +402,8 @@ class KvCache:
                 raise ValueError(f"{name} has {self.dim} elements")
         if inv_freq is not None and (inv_freq.element_size() != 8 or not inv_freq.is_floating_point() or not inv_freq.is_contiguous() or inv_freq.device != self.device):
             raise ValueError("inv_freq is a contiguous float64 tensor on the cache's device")
+        if inv_freq is not None:
+            _no_gradient("inv_freq", inv_freq)
         a = KvAppendArgs(self._data("q", q), self._data("qkv", qkv), q_stride, qkv_stride, self._ints("seqs", seqs), self._ints("starts", starts),
                          self._data("q_weight", q_weight), self._data("k_weight", k_weight), None if inv_freq is None else inv_freq.data_ptr(), eps,
                          self._entries(seqs, starts, rows), rows, heads, layer, 0 if inv_freq is None else 2 * inv_freq.numel(), interleaved)
