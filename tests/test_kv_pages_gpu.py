@@ -66,3 +66,37 @@ def test_calls_refuse_tensors_that_require_a_gradient(pk, kv):
     torch.cuda.synchronize()
     assert bool(out.any())
     c.destroy()
+
+
+def test_the_decode_cache_notices_that_its_pages_are_used_up(pk, kv):
+    """The decode workload's cache, with room for 28 tokens a request: the step that finds no room any more says so."""
+    from xsched_b200 import llama_decode as ld
+    prompt, tokens = 100, 28                                                 # to the end of a page: no slack
+    c = ld.PagedCache(torch.Generator(device="cuda").manual_seed(0), 1, prompt, 2, tokens, torch.device("cuda"))
+    seqs = _ints([1, 2])
+    c.start(seqs)
+    for _ in range(tokens):
+        c.extend(seqs)
+        c.check()
+    c.extend(seqs)
+    with pytest.raises(RuntimeError, match="too small"):
+        c.check()
+    assert c.cache.lens.tolist() == [prompt, prompt + tokens, prompt + tokens]
+    c.stop(_ints([1]))
+    c.extend(_ints([2]))
+    with pytest.raises(RuntimeError, match="too long"):
+        c.check()
+    c.cache.destroy()
+
+
+def test_the_decode_workload_looks_at_every_step(pk, kv, monkeypatch):
+    """Its loop stops with an error when a step's extend has found no room."""
+    import sys
+
+    from xsched_b200 import llama_decode as ld
+    monkeypatch.setattr(sys, "argv", ["llama_decode", "--requests", "3", "--tokens", "80", "--rate", "500", "--layers", "1", "--kv", "64", "--batched",
+                                      "--max-batch", "2", "--paged"])
+    make = ld.PagedCache.__init__
+    monkeypatch.setattr(ld.PagedCache, "__init__", lambda self, g, layers, prompt, slots, tokens, dev: make(self, g, layers, prompt, slots, 1, dev))
+    with pytest.raises(RuntimeError, match="too small"):
+        ld.main()

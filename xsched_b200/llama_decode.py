@@ -126,14 +126,15 @@ class PagedCache:
         self.q, self.out = (torch.empty(slots, NQ, HD, device=dev, dtype=torch.bfloat16) for _ in range(2))
         self.scratch = torch.zeros(self.cache.attention_scratch_bytes(slots, slots, NQ), dtype=torch.uint8, device=dev)
         self.cache.extend(self.prompt, self.shared, self._stream())
-        self._settled(self.cache.result(self._stream()))
+        self.check()
 
     @staticmethod
     def _stream():
         return torch.cuda.current_stream().cuda_stream
 
-    @staticmethod
-    def _settled(report):
+    def check(self):
+        """Whether the last extend had room: it changes nothing without, and the step's tokens fell on those of the step before."""
+        report = self.cache.result(self._stream())
         if report.missing or report.refused:
             raise RuntimeError(f"the page pool is too small: {report.missing} pages missing, {report.refused} sequences too long")
 
@@ -214,7 +215,10 @@ def main() -> None:
                     for l in layers:
                         x = l.batched(x, rows_all[:n], pos)
                 xb[:n] = x
-                return logits_of(x)
+                tokens = logits_of(x)
+                if kv is not None:
+                    kv.check()                            # the stream has just been waited for
+                return tokens
 
             for n in list(range(1, a.max_batch + 1)) * 2:                      # warm-up: every batch size once picks its kernels
                 if kv is None:
