@@ -219,3 +219,16 @@ def test_calls_and_grids_of_any_size_write_the_same_bytes(pk, kv):
         assert torch.equal(out, want)
     t.destroy()
     c.destroy()
+
+
+@pytest.mark.parametrize("dtype, group, heads, dim, page", [("bf16", 33, 1, 64, 16), ("fp16", 64, 2, 128, 64), ("bf16", 100, 1, 128, 128), ("fp16", 129, 1, 64, 32),
+                                                            ("bf16", 300, 1, 64, 64)])
+@pytest.mark.parametrize("shared", [None, 256])
+def test_many_query_heads_on_one_key_head(pk, kv, dtype, group, heads, dim, page, shared):
+    """A single token has more rows than a unit takes: tiles, direct and merged, with up to 128 rows and with more."""
+    lens = [300, 257, 1200, 400]
+    c = _filled(pk, lens, page, heads, dim, TYPES[dtype])
+    _share(c, lens, 256)
+    q = _normal(_gen(46), TYPES[dtype], 4, heads * group, dim, scale=2.0)
+    _check(kv, c, q, _attend(pk, c, q, None, None, 4, shared=shared), list(range(4)), list(range(5)))
+    c.destroy()
