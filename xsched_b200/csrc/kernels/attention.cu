@@ -47,7 +47,7 @@ __device__ __forceinline__ int warp_claim(Ctl *ctl, const AttnShared *sh, int wh
     return __shfl_sync(0xffffffffu, t, 0);
 }
 
-// An item from the loader; all lanes of a warp, or the issuing thread alone.
+// An item from the loader; all lanes of a warp.
 __device__ __forceinline__ int next_item(AttnShared *sh, Ctl *ctl, uint32_t &seen) {
     const uint32_t slot = seen % kSched;
     if (!wait_bar(&sh->item_full[slot], (seen / kSched) & 1u, sh, ctl, kErrAttnTile)) return kStopped;

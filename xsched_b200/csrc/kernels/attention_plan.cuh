@@ -10,7 +10,8 @@ constexpr int kWorkers = 8;                                 // warps that run un
 constexpr int kUnitThreads = kWorkers * 32;
 constexpr int kAttnThreads = kUnitThreads + 128;            // and a third group for tiles: one warp loads, one issues MMAs
 // Registers: 384 threads are launched with 168 each; the workers, whose rows of scores fill 128, take over what the helpers
-// do not need: 2 * 216 + 72 = 3 * 168.
+// do not need: 2 * 216 + 72 = 3 * 168.  The forms with tiles spill all the same (724 bytes of stores at head_dim 128, 352 at 64: units and
+// tiles in one kernel); the forms without take up to 224 registers and spill nothing.
 constexpr int kWorkerRegs = 216, kHelperRegs = 72;
 static_assert(2 * kWorkerRegs + kHelperRegs <= 3 * 168, "more registers than the launch has");
 constexpr int kBlock = 16;                                  // positions per block of a unit
@@ -35,7 +36,9 @@ constexpr int kShareRows = 64;
 constexpr int kMergeRowsMost = 32;
 constexpr int kPageWords = 16;                              // more than the steps that a ring holds
 constexpr int kSched = 2;                                   // items the loader may be ahead
-constexpr float kTileUs = 2.6f;                             // measured time of a tile of 256 rows at head_dim 128
+// Time of a tile of 256 rows at head_dim 128 that the cut reckons with, from an earlier form of the loop.  It scales it by head_dim, which the
+// tiles do not bear out: they take 3.0 us at 64 and at 128 (prompts of 1024 on 8192).
+constexpr float kTileUs = 2.6f;
 constexpr uint32_t kErrAttnLoad  = 0x70000001u;
 constexpr uint32_t kErrAttnMerge = 0x70000002u;
 constexpr uint32_t kErrAttnTile  = 0x70000003u;
@@ -164,7 +167,8 @@ __device__ __forceinline__ bool by_tiles(const SeqPlan &p, uint32_t group) { ret
 __device__ __forceinline__ int row_groups(long long rows) { return (int)((rows + kUnitRows - 1) / kUnitRows); }
 __device__ __forceinline__ int row_tiles(long long rows) { return (int)((rows + kItemRows - 1) / kItemRows); }
 // With at most 128 rows the two groups of workers take half of a run's tiles each, and leave a result each; where so many results
-// do not fit the scratch (half_rows 0) the first group takes all of them.
+// do not fit the scratch (half_rows 0) the first group takes all of them.  Sequences of 64 rows by halves and without: 64 of 8000
+// positions 542 and 581 us; but 256 of 500 positions 686 and 331 us, where the merges outweigh what halves gain.
 __device__ __forceinline__ int halves(const AttnShared *sh, long long rows) { return rows <= sh->half_rows ? 2 : 1; }
 __device__ __forceinline__ int chunks(int positions, int each, int run) { return max(1, ((positions + each - 1) / each + run - 1) / run); }
 __device__ __forceinline__ int tiles_of(int positions) { return (positions + kTile - 1) / kTile; }

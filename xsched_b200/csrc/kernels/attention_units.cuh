@@ -3,7 +3,8 @@
 // A unit is HBM-bound: 2 * 16 * head_dim * 2 bytes per block for 4 * 16 * 16 * head_dim flop.  Each warp has a ring of
 // blocks of its own in shared memory, filled by TMA (128-byte swizzle) ahead of use.  Scores are computed transposed,
 // S^T = K Q^T with mma.m16n8k16 (positions are M, 8 rows are N), so that up to 8 rows cost one MMA column block, and
-// O^T = V^T P^T; the C fragment of S^T becomes the B fragment of P^T by transposing its 8x8 quarters (movmatrix).
+// O^T = V^T P^T; the C fragment of S^T becomes the B fragment of P^T by transposing its 8x8 quarters (movmatrix).  P is rounded to the
+// cache's 16-bit type for the second product, as in the tiles; sums and products are fp32.
 #pragma once
 #include "attention_plan.cuh"
 

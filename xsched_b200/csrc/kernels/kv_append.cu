@@ -207,7 +207,7 @@ __global__ void __launch_bounds__(kAppendThreads, 3) kv_append_kernel(CacheView 
 template <class T, int kLanes>
 static void launch_rows(const CacheView &c, const xpkKvAppendArgs &a, int sms, cudaStream_t st) {
     // Four rows a CTA share one search, one set of look-ups and fill the threads with angles, where there are rows enough for every
-    // SM to have several CTAs of them (11,100 rows, 273 MB in and out: 66 us against 80 with one row a CTA); fewer are spread, one a CTA.
+    // SM to have several CTAs of them (11,100 rows, 273 MB in and out: 70 us against 84 with one row a CTA); fewer are spread, one a CTA.
     if (a.rows >= (uint32_t)sms * 8) kv_append_kernel<T, kLanes, 4><<<(a.rows + 3) / 4, kAppendThreads, 0, st>>>(c, a);
     else kv_append_kernel<T, kLanes, 1><<<a.rows, kAppendThreads, 0, st>>>(c, a);
 }
